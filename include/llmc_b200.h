@@ -348,6 +348,73 @@ llmc_status llmc_awq_search(llmc_ctx* ctx, const void* W, int32_t dtype, int64_t
                             const float* act_max, int32_t n_grid, const llmc_qconfig* cfg, float* best_s,
                             double* mse_out, int32_t* best_k);
 
+/* ---- products and lookups with packed 4-bit weights, embedding (extensions) ---------------------
+ * No reference counterpart: the reference dequantises packed weights (Int4PackedTensor.cs:152-161)
+ * and leaves the model's forward to the caller (GPTQModifier.cs:98-104).  These run a compressed
+ * model from the codes that the GPTQ / RTN entry points write, and its embedding.
+ *
+ * They differ from the calls above in three points, so that several threads, streams and captured
+ * graphs can share one context: `stream` is the cudaStream_t they run on (NULL: the context's; the
+ * legacy default stream is (void*)0x1); scratch is the caller's (`ws`, 256-byte aligned, of the size
+ * the matching *_workspace call gives, not shared by calls that may overlap); the calling thread's
+ * current device is given back.  They only enqueue work, and may be captured. */
+
+/* A weight [rows, cols] of 4-bit codes laid out by llmc_int4_layout; all pointers are device
+ * memory of the caller.  W[n][k] = (u - zero) * scale, u in [0, 15], zero the zero-point of an
+ * asymmetric grid or 8. */
+typedef struct {
+    const uint32_t* packed; /* 128 x 128 tiles of 8 KB, rows and columns rounded up */
+    const float* scales;    /* [groups][rows rounded up to 128] */
+    const uint8_t* zeros;   /* the same shape */
+    const int32_t* exps;    /* powers of two of the scales' largest value, per row and per group */
+    int64_t rows, cols;
+    int64_t group_size;     /* columns per scale; >= cols: one scale per row */
+} llmc_int4_weight;
+
+/* Elements of packed, of scales (and zeros), and of exps.  group_size >= 16, or >= cols. */
+llmc_status llmc_int4_layout_sizes(int64_t rows, int64_t cols, int64_t group_size, int64_t* packed_words,
+                                   int64_t* entries, int64_t* exps);
+/* Lays out one weight's codes as the GPTQ / RTN entry points write them for num_bits <= 4
+ * ((q - zp) & 0xF, two per byte, even column high, crow bytes per row), with the scales and int32
+ * zero-points (0..15; may be NULL when symmetric) of `strategy`, into w's arrays.  For TENSOR and
+ * CHANNEL w->group_size is >= cols. */
+llmc_status llmc_int4_layout(llmc_ctx* ctx, void* stream, const uint8_t* codes, int64_t crow, const float* scales,
+                             const int32_t* zps, int32_t strategy, int32_t symmetric, const llmc_int4_weight* w);
+/* out [rows, ldo] = W, each (u - zero) * scale in fp32 rounded once to dtype. */
+llmc_status llmc_int4_dequantize(llmc_ctx* ctx, void* stream, const llmc_int4_weight* w, int32_t dtype, void* out,
+                                 int64_t ldo);
+/* y [tokens, ldy] = x [tokens, ldx] W^T + bias (bias [rows], may be NULL), all of dtype.  Sums in fp32,
+ * one rounding.  Up to 16 tokens the codes enter as exact integers; above, and in the gradient, W is
+ * rounded to a 16-bit dtype first, or kept to 24 bits for F32. */
+llmc_status llmc_int4_linear_workspace(llmc_ctx* ctx, const llmc_int4_weight* w, const void* x, int32_t dtype,
+                                       int64_t tokens, int64_t ldx, int64_t* bytes);
+llmc_status llmc_int4_linear(llmc_ctx* ctx, void* stream, const llmc_int4_weight* w, const void* x, int32_t dtype,
+                             int64_t tokens, int64_t ldx, const void* bias, void* y, int64_t ldy, void* ws,
+                             int64_t ws_bytes);
+/* dx [tokens, lddx] = dy [tokens, lddy] W. */
+llmc_status llmc_int4_linear_grad_workspace(llmc_ctx* ctx, const llmc_int4_weight* w, const void* dy, int32_t dtype,
+                                            int64_t tokens, int64_t lddy, int64_t* bytes);
+llmc_status llmc_int4_linear_grad(llmc_ctx* ctx, void* stream, const llmc_int4_weight* w, const void* dy, int32_t dtype,
+                                  int64_t tokens, int64_t lddy, void* dx, int64_t lddx, void* ws, int64_t ws_bytes);
+/* out [cols] = column sums of x [rows, ld] in fp32, rounded once (a bias's gradient). */
+llmc_status llmc_col_sum_workspace(llmc_ctx* ctx, int64_t rows, int64_t cols, int64_t* bytes);
+llmc_status llmc_col_sum(llmc_ctx* ctx, void* stream, const void* x, int32_t dtype, int64_t rows, int64_t cols,
+                         int64_t ld, void* out, void* ws, int64_t ws_bytes);
+/* out [tokens, ldo] = scale * table[ids], rounded once; ids int64 (ids64 = 1) or int32.  An id outside
+ * [0, vocab) gives a row of zeros; the next llmc_sync reports it as LLMC_ERR_OUT_OF_RANGE. */
+llmc_status llmc_embedding(llmc_ctx* ctx, void* stream, const void* ids, int32_t ids64, int64_t tokens, const void* table,
+                           int32_t dtype, int64_t vocab, int64_t hidden, int64_t ldt, float scale, void* out, int64_t ldo);
+/* The same from a packed table, in dtype. */
+llmc_status llmc_int4_embedding(llmc_ctx* ctx, void* stream, const void* ids, int32_t ids64, int64_t tokens,
+                                const llmc_int4_weight* w, int32_t dtype, float scale, void* out, int64_t ldo);
+/* dtable [vocab, hidden] (contiguous, all of it written) = scale * sum of the dy rows of each id, in token
+ * order, in fp32, rounded once to dtype: two calls give the same bits.  The row padding_idx (-1: none) gets zeros, ids
+ * outside the table no part. */
+llmc_status llmc_embedding_grad_workspace(llmc_ctx* ctx, int64_t tokens, int64_t vocab, int64_t hidden, int64_t* bytes);
+llmc_status llmc_embedding_grad(llmc_ctx* ctx, void* stream, const void* ids, int32_t ids64, int64_t tokens, const void* dy,
+                                int32_t dtype, int64_t lddy, int64_t vocab, int64_t hidden, float scale,
+                                int64_t padding_idx, void* dtable, void* ws, int64_t ws_bytes);
+
 #if defined(__GNUC__)
 #pragma GCC visibility pop
 #endif

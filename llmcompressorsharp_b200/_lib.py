@@ -40,6 +40,20 @@ class QConfig(C.Structure):
     ]
 
 
+class Int4WeightC(C.Structure):
+    """llmc_int4_weight."""
+
+    _fields_ = [
+        ("packed", C.c_void_p),
+        ("scales", C.c_void_p),
+        ("zeros", C.c_void_p),
+        ("exps", C.c_void_p),
+        ("rows", C.c_int64),
+        ("cols", C.c_int64),
+        ("group_size", C.c_int64),
+    ]
+
+
 P = C.c_void_p
 I32, I64, F32 = C.c_int32, C.c_int64, C.c_float
 
@@ -90,6 +104,19 @@ _SIGS = {
     "llmc_act_absmax": [P, P, I32, I64, I64, I64, P, I32],
     "llmc_smooth_apply": [P, P, P, I32, P, I32, I64, I64, F32, P],
     "llmc_scale_apply": [P, P, P, I32, P, I32, I64, I64],
+    "llmc_int4_layout_sizes": [I64, I64, I64, C.POINTER(I64), C.POINTER(I64), C.POINTER(I64)],
+    "llmc_int4_layout": [P, P, P, I64, P, P, I32, I32, P],
+    "llmc_int4_dequantize": [P, P, P, I32, P, I64],
+    "llmc_int4_linear_workspace": [P, P, P, I32, I64, I64, C.POINTER(I64)],
+    "llmc_int4_linear": [P, P, P, P, I32, I64, I64, P, P, I64, P, I64],
+    "llmc_int4_linear_grad_workspace": [P, P, P, I32, I64, I64, C.POINTER(I64)],
+    "llmc_int4_linear_grad": [P, P, P, P, I32, I64, I64, P, I64, P, I64],
+    "llmc_col_sum_workspace": [P, I64, I64, C.POINTER(I64)],
+    "llmc_col_sum": [P, P, P, I32, I64, I64, I64, P, P, I64],
+    "llmc_embedding": [P, P, P, I32, I64, P, I32, I64, I64, I64, F32, P, I64],
+    "llmc_int4_embedding": [P, P, P, I32, I64, P, I32, F32, P, I64],
+    "llmc_embedding_grad_workspace": [P, I64, I64, I64, C.POINTER(I64)],
+    "llmc_embedding_grad": [P, P, P, I32, I64, P, I32, I64, I64, I64, F32, I64, P, P, I64],
     "llmc_awq_search": [P, P, I32, I64, I64, I64, P, I32, C.POINTER(QConfig), P, P, P],
 }
 
@@ -135,13 +162,11 @@ def call(name: str, *args) -> None:
         raise_for_status(st, f"{name}: {last_error()}")
 
 
-def ctx_for(device_index: int) -> int:
-    """Per-device context handle (created on first use), bound to torch's current stream."""
-    import torch
-
-    lib = load()
+def ctx_handle(device_index: int) -> int:
+    """Per-device context handle (created on first use)."""
     h = _ctxs.get(device_index)
     if h is None:
+        lib = load()
         with _lock:
             h = _ctxs.get(device_index)
             if h is None:
@@ -151,10 +176,27 @@ def ctx_for(device_index: int) -> int:
                     raise_for_status(st, f"llmc_init: {last_error()}")
                 h = out.value
                 _ctxs[device_index] = h
+    return h
+
+
+def stream(device_index: int) -> int:
+    """torch's current stream on a device, for the calls that take their stream.  torch reports the
+    legacy default stream as handle 0; it is passed as cudaStreamLegacy (0x1), because NULL is the
+    context's own stream."""
+    import torch
+
+    return torch._C._cuda_getCurrentRawStream(device_index) or CUDA_STREAM_LEGACY
+
+
+def ctx_for(device_index: int) -> int:
+    """Per-device context handle (created on first use), bound to torch's current stream."""
+    import torch
+
+    h = ctx_handle(device_index)
     # torch reports the legacy default stream as handle 0; pass it as cudaStreamLegacy
     # (0x1) so the library's kernels are ordered with torch's work on that stream.
     stream = torch.cuda.current_stream(device_index).cuda_stream or CUDA_STREAM_LEGACY
-    st = lib.llmc_set_stream(h, P(stream))
+    st = load().llmc_set_stream(h, P(stream))
     if st != 0:
         raise_for_status(st, f"llmc_set_stream: {last_error()}")
     return h

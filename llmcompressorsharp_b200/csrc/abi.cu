@@ -93,14 +93,16 @@ llmc_status injected_fault(const char* fn) {
 // Synchronises the stream and reports the device error words, clearing them: word 2, a bounded
 // device wait that gave up (written by the tensor-core kernels), as LLMC_ERR_TIMEOUT; word 3, a
 // Hessian that was not positive definite in a factorisation run with deferred errors, as
-// LLMC_ERR_NOT_PD.
-llmc_status device_error_check(llmc_ctx* ctx) {
-    LLMC_CUDA_TRY(cudaMemcpyAsync(ctx->hflags + 2, ctx->dflags + 2, 2 * sizeof(int), cudaMemcpyDeviceToHost, ctx->stream));
+// LLMC_ERR_NOT_PD; and for llmc_sync (ids) word 4, an embedding id outside its table, as
+// LLMC_ERR_OUT_OF_RANGE.
+llmc_status device_error_check(llmc_ctx* ctx, bool ids) {
+    const int words = ids ? 3 : 2;
+    LLMC_CUDA_TRY(cudaMemcpyAsync(ctx->hflags + 2, ctx->dflags + 2, words * sizeof(int), cudaMemcpyDeviceToHost, ctx->stream));
     LLMC_CUDA_TRY(cudaStreamSynchronize(ctx->stream));
-    const int timeout = ctx->hflags[2], not_pd = ctx->hflags[3];
-    if (timeout || not_pd) {
-        ctx->hflags[2] = ctx->hflags[3] = 0;
-        LLMC_CUDA_TRY(cudaMemsetAsync(ctx->dflags + 2, 0, 2 * sizeof(int), ctx->stream));
+    const int timeout = ctx->hflags[2], not_pd = ctx->hflags[3], bad_id = ids ? ctx->hflags[4] : 0;
+    if (timeout || not_pd || bad_id) {
+        ctx->hflags[2] = ctx->hflags[3] = ctx->hflags[4] = 0;
+        LLMC_CUDA_TRY(cudaMemsetAsync(ctx->dflags + 2, 0, words * sizeof(int), ctx->stream));
     }
     if (timeout)
         return fail(LLMC_ERR_TIMEOUT, "a bounded wait inside a tensor-core kernel gave up; results of the "
@@ -109,6 +111,9 @@ llmc_status device_error_check(llmc_ctx* ctx) {
         return fail(LLMC_ERR_NOT_PD, "a damped Hessian factorised with deferred errors was not positive definite "
                     "(its factor was written as zeros); the pseudo-inverse fallback runs on the synchronous "
                     "path: factor it again with deferred errors off");
+    if (bad_id)
+        return fail(LLMC_ERR_OUT_OF_RANGE, "an embedding id was outside its table; its rows were written as zeros and "
+                    "took no part in the gradient");
     return LLMC_OK;
 }
 
@@ -213,10 +218,16 @@ llmc_status llmc_init(int32_t device, llmc_ctx** out) {
     if (!c) return fail(LLMC_ERR_INTERNAL, "out of host memory");
     c->device = device;
     c->sm_count = prop.multiProcessorCount;
+    // The first call on a device may come while one of the caller's streams is being captured: the
+    // allocations belong to no graph, and nothing is put on the capturing or the legacy stream.
+    cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+    cudaThreadExchangeStreamCaptureMode(&mode);
     cudaError_t e = cudaStreamCreateWithFlags(&c->own_stream, cudaStreamNonBlocking);
     if (e == cudaSuccess) e = cudaMalloc(&c->dflags, 16 * sizeof(int));
-    if (e == cudaSuccess) e = cudaMemset(c->dflags, 0, 16 * sizeof(int));
+    if (e == cudaSuccess) e = cudaMemsetAsync(c->dflags, 0, 16 * sizeof(int), c->own_stream);
+    if (e == cudaSuccess) e = cudaStreamSynchronize(c->own_stream);
     if (e == cudaSuccess) e = cudaMallocHost(&c->hflags, 16 * sizeof(int));
+    cudaThreadExchangeStreamCaptureMode(&mode);
     if (e != cudaSuccess) {
         if (c->own_stream) cudaStreamDestroy(c->own_stream);
         if (c->dflags) cudaFree(c->dflags);
@@ -276,7 +287,7 @@ llmc_status llmc_set_deferred_errors(llmc_ctx* ctx, int32_t on) {
 llmc_status llmc_sync(llmc_ctx* ctx) {
     LLMC_ENTRY();
     CTX_CHECK(ctx);
-    return device_error_check(ctx);
+    return device_error_check(ctx, true);
 }
 
 llmc_status llmc_launch_count(llmc_ctx* ctx, int64_t* out) {

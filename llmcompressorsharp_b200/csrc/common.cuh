@@ -110,7 +110,8 @@ struct Carver {
 };
 
 inline llmc_status check_launch(llmc_ctx* ctx, const char* what) {
-    ctx->launches++;
+    // counted atomically: calls that take their own stream may come from several threads
+    __atomic_fetch_add(&ctx->launches, 1, __ATOMIC_RELAXED);
     cudaError_t e = cudaGetLastError();
     if (e != cudaSuccess) return fail(LLMC_ERR_CUDA, "launch of %s failed: %s", what, cudaGetErrorString(e));
     return LLMC_OK;

@@ -1,0 +1,693 @@
+// Products of many rows with a packed 4-bit weight on the 5th-generation tensor cores:
+//
+//   forward   y[t][n]  = sum_k x[t][k] W[n][k] + b[n]
+//   gradient  dx[t][k] = sum_n dy[t][n] W[n][k]
+//
+// The activations (A, K-major) come by TMA; the weight (B) is dequantised by eight warps straight into the
+// shared memory the MMA reads: K-major for the forward product (rows n, 64 columns k to a stage), MN-major for
+// the gradient (rows n are the contraction, 128 columns k to a CTA), so one copy of the codes serves both and
+// no 16-bit weight is ever written to memory.
+//
+// W in 16 bits.  (u - z) s is rounded once to the activations' type (2^-8 relative at most in bf16, 2^-11 in fp16): the
+// scale goes in as a sum of two 16-bit numbers, fma(v, s_hi, v s_lo), v an exact integer.  That is the weight
+// that the quantisers themselves hand back in a model of that type (FakeQuantizeFunction.cs:39-44 rounds its
+// last product to the tensor's type), and it lets a product run over any group size without leaving TMEM.  In
+// fp16 the scales are first brought near one by a power of two per row (forward) or per group (gradient) that
+// the epilogue takes back in fp32, so small scales keep their bits.
+//
+// fp32 activations come as three bf16 pieces that add up to them exactly; W is split the same way after its
+// product in fp32, and the six piece products down to 2^-24 are added, small ones first.  Tensor-core fp32
+// accumulation truncates, so TMEM then holds 256 terms of the contraction at most before the epilogue adds them
+// to fp32 registers.
+//
+// A persistent grid of CTA pairs (256 tokens x 256 columns, cta_group::2) or, for up to 128 tokens and for fp32,
+// single CTAs (128 x 128).  Per CTA: a TMA warp, an MMA warp, epilogue warps, eight dequantising warps, a ring of
+// STAGES x (16 KB activations + 16 KB weights), two accumulators in TMEM.  Every wait is bounded.
+#include "int4.cuh"
+#include "ops.h"
+#include "tc_common.cuh"
+
+#include <cuda.h>
+
+#include <mutex>
+
+namespace llmc {
+namespace {
+
+using namespace tc;
+using namespace w4;
+
+constexpr int BK = 64, STAGES = 6;
+constexpr int A_BYTES = 128 * BK * 2, B_BYTES = 128 * BK * 2, STAGE_BYTES = A_BYTES + B_BYTES;
+constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + 1024 + 256;
+constexpr int DQ_WARPS = 8;
+constexpr int FOLD_KB = 4;  // k-blocks between folds (fp32)
+
+struct GemmInt4 {
+    View v;
+    int64_t tokens;
+    int64_t ocols;           // columns of the output
+    int tiles_m, tiles_n, splits, kb_total, kb_per, group_m;
+    int64_t piece_rows;      // rows between the pieces of the activations' map
+    const void* bias;
+    void* out;
+    int64_t ldo;
+    float* part;             // [splits][tokens][ocols] when splits > 1
+    int wide;
+    int* err;
+    uint32_t wait_limit;
+    uint32_t idesc;
+};
+
+struct Unit {
+    int64_t m0, n0;  // first token and column of the tile
+    int kb0, kb1, split;
+};
+
+template <int CG> __device__ __forceinline__ Unit unit_at(const GemmInt4& a, int u) {
+    const int tiles = a.tiles_m * a.tiles_n;
+    const int t = u % tiles;
+    Unit r;
+    r.split = u / tiles;
+    // group_m token tiles wide strips, so that the tiles in flight share both operands through L2
+    const int per = a.group_m * a.tiles_n, g = t / per, first = g * a.group_m, gm = min(a.group_m, a.tiles_m - first), l = t - g * per;
+    r.m0 = (int64_t)(first + l % gm) * (128 * CG);
+    r.n0 = (int64_t)(l / gm) * (128 * CG);
+    r.kb0 = r.split * a.kb_per;
+    r.kb1 = min(a.kb_total, r.kb0 + a.kb_per);
+    return r;
+}
+
+// The six products of pieces, small ones first: x piece (3: the first without infinities and NaN), w piece.
+constexpr int COMBOS = 6;
+__device__ __forceinline__ void combo(int c, int& xp, int& wp) {
+    xp = c == 0 ? 2 : (c == 2 || c == 3) ? 1 : c == 5 ? 0 : 3;
+    wp = c == 1 ? 2 : (c == 2 || c == 4) ? 1 : 0;
+}
+
+// One stage's codes of one thread with their scales: forward, 64 columns of one row (granules 2); gradient, 64
+// columns (chunks 2 hh, 2 hh + 1) of one row (granules 4).
+struct Frag {
+    uint32_t w[8];
+    float s[4];
+    uint8_t z[4];
+};
+
+template <int DIR>
+__device__ __forceinline__ void load_frag(const View& v, int64_t n0, int kb, int tid, Frag& f) {
+    if constexpr (DIR == 0) {
+        const int64_t n = n0 + tid;
+        const int kt = kb >> 1, h = kb & 1;
+        const uint2* p = reinterpret_cast<const uint2*>(v.packed + ((n / TILE) * (v.kp / TILE) + kt) * TILE_WORDS + (n % TILE) * 16 + 2 * h);
+#pragma unroll
+        for (int t = 0; t < 4; t++) {
+            const uint2 q = __ldg(p + 2 * t);
+            f.w[2 * t] = q.x;
+            f.w[2 * t + 1] = q.y;
+        }
+#pragma unroll
+        for (int c = 0; c < 2; c++) {
+            if (c && v.gsv % 64 == 0) {
+                f.s[1] = f.s[0];
+                f.z[1] = f.z[0];
+                break;
+            }
+            const int64_t o = (int64_t)group_of(kb * BK + 32 * c, v.gsv, v.groups) * v.mp + n;
+            f.s[c] = __ldg(v.scales + o);
+            f.z[c] = __ldg(v.zeros + o);
+        }
+    } else {
+        const int64_t n = (int64_t)kb * BK + tid % 64;
+        const int hh = tid / 64;
+        const uint4* p = reinterpret_cast<const uint4*>(v.packed + ((n / TILE) * (v.kp / TILE) + n0 / TILE) * TILE_WORDS + (n % TILE) * 16) + 2 * hh;
+#pragma unroll
+        for (int q = 0; q < 2; q++) {
+            const uint4 x = __ldg(p + q);
+            f.w[4 * q] = x.x;
+            f.w[4 * q + 1] = x.y;
+            f.w[4 * q + 2] = x.z;
+            f.w[4 * q + 3] = x.w;
+        }
+#pragma unroll
+        for (int c = 0; c < 4; c++) {
+            if (c && v.gsv % 128 == 0) {
+                f.s[c] = f.s[0];
+                f.z[c] = f.z[0];
+                continue;
+            }
+            const int64_t o = (int64_t)group_of((int)n0 + 32 * c, v.gsv, v.groups) * v.mp + n;
+            f.s[c] = __ldg(v.scales + o);
+            f.z[c] = __ldg(v.zeros + o);
+        }
+    }
+}
+
+// Eight weights of a word in T: rounded once, or piece wp of their fp32 value.
+template <typename T, int PIECES>
+__device__ __forceinline__ uint4 dequant(uint32_t word, float s, uint32_t z, int wp) {
+    uint32_t o[4];
+    const uint32_t zz = zero_pair<T>(z);
+    if constexpr (PIECES == 1) {
+        const T hi = from_f<T>(s);
+        const T lo = from_f<T>(__fsub_rn(s, to_f<T>(hi)));
+        typename Num<T>::T2 hi2, lo2;
+        hi2.x = hi2.y = hi;
+        lo2.x = lo2.y = lo;
+#pragma unroll
+        for (int p = 0; p < 4; p++) {
+            const auto v = as2<T>(int_pair<T>(word, p, zz));
+            o[p] = bits2(__hfma2(v, hi2, __hmul2(v, lo2)));
+        }
+    } else {
+#pragma unroll
+        for (int p = 0; p < 4; p++) {
+            const uint32_t v = int_pair<T>(word, p, zz);
+            uint32_t r = 0;
+#pragma unroll
+            for (int j = 0; j < 2; j++) {
+                const float i = __uint_as_float(j ? (v & 0xFFFF0000u) : (v << 16));
+                float w = __fmul_rn(i, s);
+                __nv_bfloat16 b = __float2bfloat16_rn(w);
+                for (int q = 0; q < wp; q++) {
+                    w = __fsub_rn(w, __bfloat162float(b));
+                    b = __float2bfloat16_rn(w);
+                }
+                r |= (uint32_t)__bfloat16_as_ushort(b) << (16 * j);
+            }
+            o[p] = r;
+        }
+    }
+    return make_uint4(o[0], o[1], o[2], o[3]);
+}
+
+template <typename T, int DIR, int PIECES>
+__device__ __forceinline__ void store_frag(const Frag& f, unsigned char* b, int tid, int wp, const int* e) {
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+        int c, off;
+        if constexpr (DIR == 0) {
+            const int t = i / 2;
+            c = i % 2;
+            off = tid * 128 + (((4 * c + t) ^ (tid & 7)) << 4);
+        } else {
+            const int t = 2 * (tid / 64) + i / 4, r = tid % 64;
+            c = i % 4;
+            off = (c / 2) * (64 * BK * 2) + r * 128 + (((4 * (c & 1) + t) ^ (r & 7)) << 4);
+        }
+        float s = f.s[c];
+        if constexpr (sizeof(T) == 2 && PIECES == 1)
+            if (Num<T>::MAGIC == Num<__half>::MAGIC) s *= pow2(-e[DIR == 0 ? 0 : c]);
+        *reinterpret_cast<uint4*>(b + off) = dequant<T, PIECES>(f.w[i], s, f.z[c], wp);
+    }
+}
+
+template <int CG> __device__ __forceinline__ void commit(uint64_t* bar) {
+    if constexpr (CG == 2) umma2_commit_mc(bar, 0x3);
+    else umma_commit(bar);
+}
+
+// T: operand type; O: output (and bias) type; DIR 0 forward, 1 gradient; CG CTAs per tile; PIECES 1, or 3 for fp32.
+template <typename T, typename O, int DIR, int CG, int PIECES>
+__global__ void __launch_bounds__(32 * (2 + (PIECES == 3 ? 8 : 4) + DQ_WARPS), 1)
+    gemm_int4_kernel(const __grid_constant__ CUtensorMap amap, const __grid_constant__ GemmInt4 a) {
+    constexpr bool FOLD = PIECES == 3;
+    constexpr int EW = FOLD ? 8 : 4;          // epilogue warps
+    constexpr int BN = 128 * CG;              // columns of a tile
+    constexpr int TMEM_COLS = 2 * BN;
+    constexpr int EC = BN * 4 / EW;           // columns per epilogue warp
+    extern __shared__ unsigned char smem_raw[];
+    unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    uint64_t* afull = reinterpret_cast<uint64_t*>(smem + STAGES * STAGE_BYTES);
+    uint64_t* bfull = afull + STAGES;
+    uint64_t* empty = bfull + STAGES;
+    uint64_t* tfull = empty + STAGES;
+    uint64_t* tempty = tfull + 2;
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tempty + 2);
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+
+    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+    const uint32_t rank = CG == 2 ? cluster_ctarank() : 0;
+    const int worker = blockIdx.x / CG, workers = gridDim.x / CG;
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < STAGES; s++) {
+            mbar_init(&afull[s], 1);
+            mbar_init(&bfull[s], 4 * CG);
+            mbar_init(&empty[s], 1);
+        }
+        for (int b = 0; b < 2; b++) {
+            mbar_init(&tfull[b], 1);
+            mbar_init(&tempty[b], EW * CG);
+        }
+        *abort_flag = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 0) {
+        if constexpr (CG == 2) {
+            asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(TMEM_COLS));
+            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;");
+        } else {
+            asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(TMEM_COLS));
+            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+        }
+    }
+    tc_fence_before();
+    if constexpr (CG == 2) cluster_sync();
+    else __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = *tmem_slot;
+
+    const int units = a.tiles_m * a.tiles_n * a.splits;
+    uint32_t it = 0, cc = 0;  // stages and accumulators used so far, counted alike by every role
+    int pend[STAGES];
+#pragma unroll
+    for (int s = 0; s < STAGES; s++) pend[s] = -1;
+    int commit_par[2] = {-1, -1};
+
+    // Calls body(kb, xp, wp, first, last) for each stage of a unit in ring order: first / last mark the stages that
+    // open and close an accumulator.  body returns false to stop.
+    auto stages = [&](const Unit& u, auto&& body) -> bool {
+        if constexpr (!FOLD) {
+            for (int kb = u.kb0; kb < u.kb1; kb++)
+                if (!body(kb, 0, 0, kb == u.kb0, kb == u.kb1 - 1)) return false;
+        } else {
+            for (int c0 = u.kb0; c0 < u.kb1; c0 += FOLD_KB) {
+                const int c1 = min(u.kb1, c0 + FOLD_KB);
+                for (int c = 0; c < COMBOS; c++) {
+                    int xp, wp;
+                    combo(c, xp, wp);
+                    for (int kb = c0; kb < c1; kb++)
+                        if (!body(kb, xp, wp, c == 0 && kb == c0, c == COMBOS - 1 && kb == c1 - 1)) return false;
+                }
+            }
+        }
+        return true;
+    };
+
+    if (warp == 0) {
+        if (lane == 0) {
+            // ---- TMA: this CTA's 128 tokens
+            for (int un = worker; un < units && !*abort_flag; un += workers) {
+                const Unit u = unit_at<CG>(a, un);
+                const int row = (int)(u.m0 + rank * 128);
+                const bool ok = stages(u, [&](int kb, int xp, int, bool, bool) {
+                    const int s = it % STAGES;
+                    const uint32_t ph = (it / STAGES) & 1u;
+                    if (!mbar_wait(&empty[s], ph ^ 1u, abort_flag, a.err, a.wait_limit)) return false;
+                    unsigned char* dst = smem + s * STAGE_BYTES;
+                    const int y = row + (int)(xp * a.piece_rows);
+                    if constexpr (CG == 2) {
+                        if (rank == 0) mbar_expect_tx(&afull[s], 2 * A_BYTES);
+                        tma_load_2d_pair(dst, &amap, kb * BK, y, mapa_shared(smem_u32(&afull[s]), 0));
+                    } else {
+                        mbar_expect_tx(&afull[s], A_BYTES);
+                        tma_load_2d(dst, &amap, kb * BK, y, &afull[s]);
+                    }
+                    pend[s] = (int)ph;
+                    it++;
+                    return true;
+                });
+                if (!ok) break;
+            }
+        }
+        __syncwarp();
+    } else if (warp == 1) {
+        if (lane == 0 && rank == 0) {
+            // ---- MMA
+            for (int un = worker; un < units && !*abort_flag; un += workers) {
+                const Unit u = unit_at<CG>(a, un);
+                bool open = false;
+                const bool ok = stages(u, [&](int, int, int, bool first, bool last) {
+                    const int b = (int)(cc & 1u);
+                    if (first) {
+                        if (!mbar_wait(&tempty[b], ((cc >> 1) & 1u) ^ 1u, abort_flag, a.err, a.wait_limit)) return false;
+                        tc_fence_after();
+                        open = true;
+                    }
+                    const int s = it % STAGES;
+                    const uint32_t ph = (it / STAGES) & 1u;
+                    if (!mbar_wait(&afull[s], ph, abort_flag, a.err, a.wait_limit)) return false;
+                    if (CG == 2 ? !mbar_wait_cluster(&bfull[s], ph, abort_flag, a.err, a.wait_limit)
+                                : !mbar_wait(&bfull[s], ph, abort_flag, a.err, a.wait_limit))
+                        return false;
+                    tc_fence_after();
+                    const uint32_t abase = smem_u32(smem + s * STAGE_BYTES), bbase = abase + A_BYTES;
+                    const uint32_t dst = tmem + (uint32_t)(b * BN);
+#pragma unroll
+                    for (int kk = 0; kk < BK / 16; kk++) {
+                        const uint64_t da = smem_desc_k_sw128(abase + kk * 32);
+                        const uint64_t db = DIR == 0 ? smem_desc_k_sw128(bbase + kk * 32) : smem_desc_mn_sw128(bbase + kk * 2048, 64 * BK * 2);
+                        const uint32_t acc = first && kk == 0 ? 0u : 1u;
+                        if constexpr (CG == 2) umma2_f16(dst, da, db, a.idesc, acc);
+                        else umma_f16(dst, da, db, a.idesc, acc);
+                    }
+                    commit<CG>(&empty[s]);
+                    if (last) {
+                        commit<CG>(&tfull[b]);
+                        commit_par[b] = (int)((cc >> 1) & 1u);
+                        open = false;
+                        cc++;
+                    }
+                    it++;
+                    return true;
+                });
+                if (!ok) {
+                    if (open) {  // so that the tail can wait for what was issued
+                        commit<CG>(&tfull[cc & 1u]);
+                        commit_par[cc & 1u] = (int)((cc >> 1) & 1u);
+                    }
+                    break;
+                }
+            }
+        }
+        __syncwarp();
+    } else if (warp < 2 + EW) {
+        // ---- epilogue: TMEM lane quadrant q, columns h EC ..
+        const int q = warp % 4, h = (warp - 2) / 4;
+        float acc[FOLD ? EC : 1];
+        for (int un = worker; un < units && !*abort_flag; un += workers) {
+            const Unit u = unit_at<CG>(a, un);
+            const int64_t tok = u.m0 + rank * 128 + q * 32 + lane;
+            auto emit = [&](const float (&v)[32], int c0) {  // columns n0 + c0 .. + 31 of this thread's token
+                if (tok >= a.tokens) return;
+                const int64_t col0 = u.n0 + c0;
+                float o[32];
+#pragma unroll
+                for (int i = 0; i < 32; i++) {
+                    o[i] = v[i];
+                    if constexpr (Num<T>::MAGIC == Num<__half>::MAGIC) {
+                        const int64_t col = col0 + i;
+                        if (DIR == 0) {
+                            if (col < a.v.rows) o[i] *= pow2(a.v.exps[col]);
+                        } else {
+                            if (col < a.v.kp) o[i] *= pow2(a.v.exps[a.v.mp + group_of((int)col, a.v.gsv, a.v.groups)]);
+                        }
+                    }
+                }
+                const bool part = a.splits > 1;
+                float* prow = a.part + ((int64_t)u.split * a.tokens + tok) * a.ocols;
+                O* row = reinterpret_cast<O*>(a.out) + tok * a.ldo;
+                const bool mapped = DIR == 1 && !a.v.identity;
+                if (!part && a.wide && !mapped && col0 + 32 <= a.ocols) {
+                    constexpr int N = 16 / (int)sizeof(O);
+#pragma unroll
+                    for (int i = 0; i < 32; i += N) {
+                        union { O h[N]; uint4 u4; } x;
+#pragma unroll
+                        for (int j = 0; j < N; j++) {
+                            float f = o[i + j];
+                            if (a.bias) f += to_f<O>(reinterpret_cast<const O*>(a.bias)[col0 + i + j]);
+                            x.h[j] = from_f<O>(f);
+                        }
+                        *reinterpret_cast<uint4*>(row + col0 + i) = x.u4;
+                    }
+                    return;
+                }
+                if (part && !mapped && a.ocols % 4 == 0 && col0 + 32 <= a.ocols) {
+#pragma unroll
+                    for (int i = 0; i < 32; i += 4)
+                        *reinterpret_cast<float4*>(prow + col0 + i) = make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+                    return;
+                }
+#pragma unroll
+                for (int i = 0; i < 32; i++) {
+                    int64_t col = col0 + i;
+                    if (mapped) {
+                        if (col >= a.v.kp) continue;
+                        col = column_of((int)col, a.v.gs, a.v.gsv, a.v.groups, a.v.cols);
+                        if (col < 0) continue;
+                    }
+                    if (col >= a.ocols) continue;
+                    if (part) {
+                        prow[col] = o[i];
+                    } else {
+                        float f = o[i];
+                        if (a.bias) f += to_f<O>(reinterpret_cast<const O*>(a.bias)[col]);
+                        row[col] = from_f<O>(f);
+                    }
+                }
+            };
+            const int chunks = FOLD ? (u.kb1 - u.kb0 + FOLD_KB - 1) / FOLD_KB : 1;
+            if constexpr (FOLD) {
+#pragma unroll
+                for (int i = 0; i < EC; i++) acc[i] = 0.f;
+            }
+            bool ok = true;
+            for (int c = 0; c < chunks; c++, cc++) {
+                const int b = (int)(cc & 1u);
+                const bool have = mbar_wait(&tfull[b], (cc >> 1) & 1u, abort_flag, a.err, a.wait_limit);
+                if (!__all_sync(0xffffffffu, have ? 1 : 0)) {
+                    ok = false;
+                    break;
+                }
+                tc_fence_after();
+                const uint32_t taddr = tmem + ((uint32_t)(q * 32) << 16) + (uint32_t)(b * BN + h * EC);
+#pragma unroll
+                for (int p = 0; p < EC / 32; p++) {
+                    uint32_t r[32];
+                    tmem_ld32(taddr + p * 32, r);
+                    if constexpr (FOLD) {
+#pragma unroll
+                        for (int i = 0; i < 32; i++) acc[p * 32 + i] = __fadd_rn(acc[p * 32 + i], __uint_as_float(r[i]));
+                    } else {
+                        float v[32];
+#pragma unroll
+                        for (int i = 0; i < 32; i++) v[i] = __uint_as_float(r[i]);
+                        emit(v, h * EC + p * 32);
+                    }
+                }
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) {
+                    if constexpr (CG == 2) mbar_arrive_cluster_cta(mapa_shared(smem_u32(&tempty[b]), 0));
+                    else mbar_arrive(&tempty[b]);
+                }
+            }
+            if (!ok) break;
+            if constexpr (FOLD) {
+#pragma unroll
+                for (int p = 0; p < EC / 32; p++) {
+                    float v[32];
+#pragma unroll
+                    for (int i = 0; i < 32; i++) v[i] = acc[p * 32 + i];
+                    emit(v, h * EC + p * 32);
+                }
+            }
+        }
+    } else {
+        // ---- dequantising: two groups of four warps take the 128-wide steps of the contraction in turn
+        const int grp = (warp - 2 - EW) / 4, tid = threadIdx.x - 32 * (2 + EW + 4 * grp);
+        for (int un = worker; un < units && !*abort_flag; un += workers) {
+            const Unit u = unit_at<CG>(a, un);
+            const int64_t n0 = u.n0 + rank * 128;
+            // the last tile of a pair may reach past the padded weight: its columns are never stored
+            const int64_t lim = DIR == 0 ? a.v.mp : a.v.kp;
+            const int64_t nl = n0 < lim ? n0 : lim - 128;
+            int e[4] = {0, 0, 0, 0};
+            if constexpr (Num<T>::MAGIC == Num<__half>::MAGIC) {
+                if constexpr (DIR == 0) e[0] = a.v.exps[nl + tid];
+                else
+#pragma unroll
+                    for (int c = 0; c < 4; c++) e[c] = a.v.exps[a.v.mp + group_of((int)nl + 32 * c, a.v.gsv, a.v.groups)];
+            }
+            Frag f;
+            bool have = false;
+            const bool ok = stages(u, [&](int kb, int, int wp, bool, bool) {
+                const int s = it % STAGES;
+                const uint32_t ph = (it / STAGES) & 1u;
+                it++;
+                // A group follows the ring through the other's steps too: were it to skip their waits, units with few
+                // steps could leave it a whole turn of the ring behind, where the parity means the turn before.
+                if (((kb >> 1) & 1) != grp) return mbar_wait(&empty[s], ph ^ 1u, abort_flag, a.err, a.wait_limit);
+                if (!have) load_frag<DIR>(a.v, nl, kb, tid, f);
+                const Frag cur = f;
+                // the next step of this group within the unit, fetched while this one is converted
+                int nk = (kb & 1) ? kb + 3 : kb + 1;
+                have = false;
+                if constexpr (!FOLD) {
+                    if (nk < u.kb1) {
+                        load_frag<DIR>(a.v, nl, nk, tid, f);
+                        have = true;
+                    }
+                }
+                if (!mbar_wait(&empty[s], ph ^ 1u, abort_flag, a.err, a.wait_limit)) return false;
+                store_frag<T, DIR, PIECES>(cur, smem + s * STAGE_BYTES + A_BYTES, tid, wp, e);
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                __syncwarp();
+                if (lane == 0) {
+                    if constexpr (CG == 2) mbar_arrive_cluster(mapa_shared(smem_u32(&bfull[s]), 0));
+                    else mbar_arrive(&bfull[s]);
+                }
+                return true;
+            });
+            if (!ok) break;
+        }
+    }
+
+    // Tail: no commit may still be on its way to a barrier of this CTA, nor, after an abort, a load to its memory.
+    __syncwarp();
+    if (warp == 0 && lane == 0)
+        for (int s = 0; s < STAGES; s++)
+            if (pend[s] >= 0) {
+                if (!*abort_flag) mbar_wait_drain(&empty[s], (uint32_t)pend[s]);
+                else if (rank == 0) mbar_wait_drain(&afull[s], (uint32_t)pend[s]);
+            }
+    if (*abort_flag && warp == 1 && lane == 0 && rank == 0)
+        for (int b = 0; b < 2; b++)
+            if (commit_par[b] >= 0) mbar_wait_drain(&tfull[b], (uint32_t)commit_par[b]);
+    __syncwarp();
+    tc_fence_before();
+    if constexpr (CG == 2) cluster_sync();
+    else __syncthreads();
+    if (warp == 0) {
+        tc_fence_after();
+        if constexpr (CG == 2) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(TMEM_COLS));
+        else asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(TMEM_COLS));
+    }
+}
+
+typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
+                                  const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                                  CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+EncodeTiledFn encode_fn() {
+    static const EncodeTiledFn fn = [] {
+        void* p = nullptr;
+        cudaDriverEntryPointQueryResult q;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) != cudaSuccess || q != cudaDriverEntryPointSuccess)
+            p = nullptr;
+        return reinterpret_cast<EncodeTiledFn>(p);
+    }();
+    return fn;
+}
+
+// Workers (CTAs, or pairs) of a kernel that fit the device at once; asked once per kernel and device.
+template <auto kernel> int max_workers(llmc_ctx* ctx, int cg, int threads) {
+    static std::mutex mu;
+    static int cache[64];
+    static bool known[64];
+    const int dev = ctx->device;
+    if (dev < 0 || dev >= 64) return 0;
+    std::lock_guard<std::mutex> lock(mu);
+    if (!known[dev]) {
+        int n = 0;
+        if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_BYTES) != cudaSuccess) {
+            cudaGetLastError();
+            return 0;
+        }
+        if (cg == 1) {
+            n = ctx->sm_count;
+        } else {
+            cudaLaunchConfig_t cfg = {};
+            cfg.gridDim = dim3(2 * (unsigned)ctx->sm_count);
+            cfg.blockDim = dim3((unsigned)threads);
+            cfg.dynamicSmemBytes = SMEM_BYTES;
+            cudaLaunchAttribute at[1];
+            at[0].id = cudaLaunchAttributeClusterDimension;
+            at[0].val.clusterDim.x = 2;
+            at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+            cfg.attrs = at;
+            cfg.numAttrs = 1;
+            if (cudaOccupancyMaxActiveClusters(&n, (const void*)kernel, &cfg) != cudaSuccess) {
+                cudaGetLastError();
+                n = 0;
+            }
+        }
+        cache[dev] = n;
+        known[dev] = true;
+    }
+    return cache[dev];
+}
+
+template <typename T, typename O, int DIR, int CG, int PIECES>
+llmc_status launch(llmc_ctx* ctx, cudaStream_t st, const CUtensorMap& map, GemmInt4& g) {
+    constexpr auto kernel = gemm_int4_kernel<T, O, DIR, CG, PIECES>;
+    constexpr int threads = 32 * (2 + (PIECES == 3 ? 8 : 4) + DQ_WARPS);
+    int cap = max_workers<kernel>(ctx, CG, threads);
+    const int allowed = persistent_sms(ctx) / CG;
+    if (cap > allowed) cap = allowed;
+    if (cap < 1) return fail(LLMC_ERR_CUDA, "the packed product's kernel does not fit this device");
+    const int64_t units = (int64_t)g.tiles_m * g.tiles_n * g.splits;
+    const int workers = units < cap ? (int)units : cap;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(workers * CG));
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = SMEM_BYTES;
+    cfg.stream = st;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = CG;
+    at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 1;
+    LLMC_CUDA_TRY(cudaLaunchKernelEx(&cfg, kernel, map, g));
+    return check_launch(ctx, "int4_gemm");
+}
+
+}  // namespace
+
+// CTAs per tile for a product of this many tokens and columns.
+int int4_gemm_cg(int dtype, int64_t tokens, int64_t cols) { return dtype != LLMC_DTYPE_F32 && tokens > 128 && cols > 128 ? 2 : 1; }
+
+// Splits of the contraction: enough to give every worker a tile, four k-blocks to a split at least.
+int int4_gemm_splits(const llmc_ctx* ctx, int dtype, int64_t tokens, int64_t cols, int64_t contraction) {
+    const int cg = int4_gemm_cg(dtype, tokens, cols);
+    const int64_t tile = 128 * cg, tiles = ((tokens + tile - 1) / tile) * ((cols + tile - 1) / tile);
+    const int64_t kb = (contraction + BK - 1) / BK, workers = persistent_sms(ctx) / cg;
+    int64_t s = workers / tiles;
+    if (s > kb / 4) s = kb / 4;
+    if (s > 32) s = 32;
+    if (s < 1) s = 1;
+    const int64_t per = (kb + s - 1) / s;
+    return (int)((kb + per - 1) / per);
+}
+
+// A [pieces][tokens][lda] 16-bit, K-major (see int4_stage for the pieces of fp32); out [tokens][ldo].
+llmc_status int4_gemm(llmc_ctx* ctx, cudaStream_t st, const w4::View& v, int dir, int dtype, const void* A, int64_t acols, int64_t lda,
+                      int64_t tokens, const void* bias, void* out, int64_t ldo, int splits, float* part) {
+    EncodeTiledFn enc = encode_fn();
+    if (!enc) return fail(LLMC_ERR_CUDA, "cuTensorMapEncodeTiled is not available");
+    const int pieces = dtype == LLMC_DTYPE_F32 ? 4 : 1;
+    const int64_t cols = dir == 0 ? v.rows : v.kp, contraction = dir == 0 ? v.kp : v.mp;
+    const int cg = int4_gemm_cg(dtype, tokens, cols);
+    GemmInt4 g{};
+    g.v = v;
+    g.tokens = tokens;
+    g.ocols = dir == 0 ? v.rows : v.cols;
+    const int64_t tile = 128 * cg;
+    g.tiles_m = (int)((tokens + tile - 1) / tile);
+    g.tiles_n = (int)((cols + tile - 1) / tile);
+    g.splits = splits;
+    g.kb_total = (int)(contraction / BK);
+    g.kb_per = (g.kb_total + splits - 1) / splits;
+    g.group_m = 8;
+    g.piece_rows = tokens;
+    g.bias = splits > 1 ? nullptr : bias;
+    g.out = out;
+    g.ldo = ldo;
+    g.part = part;
+    const int es = dtype_size(dtype);
+    g.wide = (uintptr_t)out % 16 == 0 && (ldo * es) % 16 == 0;
+    g.err = ctx->dflags + 2;
+    g.wait_limit = ctx->wait_limit;
+    const uint32_t fmt = dtype == LLMC_DTYPE_F16 ? 0u : 1u;
+    g.idesc = (1u << 4) | (fmt << 7) | (fmt << 10) | ((uint32_t)dir << 16) | ((uint32_t)(tile >> 3) << 17) | ((uint32_t)(tile >> 4) << 24);
+
+    CUtensorMap map;
+    const cuuint64_t dim[2] = {(cuuint64_t)acols, (cuuint64_t)(tokens * pieces)};
+    const cuuint64_t stride[1] = {(cuuint64_t)lda * 2};
+    const cuuint32_t box[2] = {BK, 128}, es1[2] = {1, 1};
+    const CUresult cr = enc(&map, fmt ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, const_cast<void*>(A), dim, stride,
+                            box, es1, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (cr != CUDA_SUCCESS) return fail(LLMC_ERR_CUDA, "cuTensorMapEncodeTiled failed (%d)", (int)cr);
+    using B = __nv_bfloat16;
+    if (dtype == LLMC_DTYPE_F32) return dir ? launch<B, float, 1, 1, 3>(ctx, st, map, g) : launch<B, float, 0, 1, 3>(ctx, st, map, g);
+    if (dtype == LLMC_DTYPE_BF16) {
+        if (cg == 2) return dir ? launch<B, B, 1, 2, 1>(ctx, st, map, g) : launch<B, B, 0, 2, 1>(ctx, st, map, g);
+        return dir ? launch<B, B, 1, 1, 1>(ctx, st, map, g) : launch<B, B, 0, 1, 1>(ctx, st, map, g);
+    }
+    if (cg == 2) return dir ? launch<__half, __half, 1, 2, 1>(ctx, st, map, g) : launch<__half, __half, 0, 2, 1>(ctx, st, map, g);
+    return dir ? launch<__half, __half, 1, 1, 1>(ctx, st, map, g) : launch<__half, __half, 0, 1, 1>(ctx, st, map, g);
+}
+
+}  // namespace llmc

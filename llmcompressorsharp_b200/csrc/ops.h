@@ -1,6 +1,7 @@
 // Internal launchers shared between the translation units of libllmc_b200.
 #pragma once
 #include "common.cuh"
+#include "int4.cuh"
 
 namespace llmc {
 
@@ -65,6 +66,36 @@ llmc_status act_quant_per_token(llmc_ctx* ctx, const void* x, int dtype, int64_t
 llmc_status ct_pack(llmc_ctx* ctx, const uint8_t* codes, int64_t m, int64_t n, int64_t crow, const int32_t* zps,
                     int64_t zrow, int64_t gs, int bits, int sym, int32_t* out, int64_t ldo, int32_t* zp_out);
 
+// ---- packed 4-bit weights (k_int4.cu, k_int4_gemm.cu) -----------------------------------------
+// These and the embedding's take their stream from the caller and use none of the context's
+// workspaces, so calls on several streams and captured ones do not share memory.
+llmc_status int4_layout(llmc_ctx* ctx, cudaStream_t st, const uint8_t* codes, int64_t crow, const float* scales,
+                        const int32_t* zps, int64_t srow, int sym, const w4::View& v, uint32_t* packed, float* sout,
+                        uint8_t* zout, int32_t* exps);
+// out[t] = scale * W[ids[t]] (ids null: row t).
+llmc_status int4_rows(llmc_ctx* ctx, cudaStream_t st, const w4::View& v, const void* ids, int ids64, int64_t tokens,
+                      float scale, void* out, int dtype, int64_t ldo);
+// x in 16 bits with rows of `pitch`, in the layout's columns (v null: in its own); fp32 in 3 or 4 bf16 pieces.
+llmc_status int4_stage(llmc_ctx* ctx, cudaStream_t st, const void* x, int dtype, int64_t tokens, int64_t n, int64_t ldx,
+                       int64_t pitch, const w4::View* v, int pieces, uint16_t* out);
+llmc_status int4_few(llmc_ctx* ctx, cudaStream_t st, const w4::View& v, const void* x, int dtype, int64_t tokens, int64_t ldx,
+                     int64_t xcols, const void* bias, void* y, int64_t ldy);
+int int4_gemm_splits(const llmc_ctx* ctx, int dtype, int64_t tokens, int64_t cols, int64_t contraction);
+llmc_status int4_gemm(llmc_ctx* ctx, cudaStream_t st, const w4::View& v, int dir, int dtype, const void* A, int64_t acols,
+                      int64_t lda, int64_t tokens, const void* bias, void* out, int64_t ldo, int splits, float* part);
+// out = sum of `splits` fp32 parts in order, + bias; and the column sums of x as parts.
+llmc_status int4_join(llmc_ctx* ctx, cudaStream_t st, const float* part, int splits, int64_t rows, int64_t cols, const void* bias,
+                      void* out, int dtype, int64_t ldo);
+llmc_status col_sum_parts(llmc_ctx* ctx, cudaStream_t st, const void* x, int dtype, int64_t rows, int64_t cols, int64_t ld,
+                          int splits, float* part);
+
+// ---- embedding (k_embedding.cu) ----------------------------------------------------------------
+llmc_status embedding_lookup(llmc_ctx* ctx, cudaStream_t st, const void* ids, int ids64, int64_t tokens, const void* table, int dtype,
+                             int64_t vocab, int64_t hidden, int64_t ldt, float scale, void* out, int64_t ldo);
+size_t embedding_grad_bytes(int64_t tokens, int64_t vocab, int64_t hidden);
+llmc_status embedding_grad(llmc_ctx* ctx, cudaStream_t st, const void* ids, int ids64, int64_t tokens, const void* dy, int dtype,
+                           int64_t lddy, int64_t vocab, int64_t hidden, float scale, int64_t padding, void* out, void* ws);
+
 // ---- GPTQ activation order (k_actorder.cu) --------------------------------------------------
 llmc_status act_order_perm(llmc_ctx* ctx, const float* H, int64_t d, int64_t ldh, int32_t* perm);
 llmc_status permute_hessian(llmc_ctx* ctx, const float* H, int64_t d, int64_t ldh, int upper_only, const int32_t* perm,
@@ -81,7 +112,7 @@ llmc_status scatter_codes(llmc_ctx* ctx, const uint8_t* src, int64_t rows, int64
 // Drops the no-allocation observer's cached device address of its static row buffer on
 // `device` (noalloc.cu); llmc_init calls it so that a reset device gets a fresh lookup.
 void noalloc_forget(int device);
-llmc_status device_error_check(llmc_ctx* ctx);
+llmc_status device_error_check(llmc_ctx* ctx, bool ids = false);
 llmc_status symmetrize_from_upper(llmc_ctx* ctx, const float* src, int64_t d, int64_t lds, float* dst, int64_t ldd);
 llmc_status convert_to_f32(llmc_ctx* ctx, const void* src, int dtype, int64_t rows, int64_t cols, int64_t lds,
                            float* dst, int64_t ldd);
