@@ -363,17 +363,14 @@ llmc_status llmc_awq_search(llmc_ctx* ctx, const void* W, int32_t dtype, int64_t
  * memory of the caller.  W[n][k] = (u - zero) * scale, u in [0, 15], zero the zero-point of an
  * asymmetric grid or 8. */
 typedef struct {
-    const uint32_t* packed; /* 128 x 128 tiles of 8 KB, rows and columns rounded up */
-    const float* scales;    /* [groups][rows rounded up to 128] */
-    const uint8_t* zeros;   /* the same shape */
-    const int32_t* exps;    /* powers of two of the scales' largest value, per row and per group */
+    const uint8_t* packed;  /* tiles of 128 x 128 codes with their scales and zeros; 16-byte aligned */
+    const int32_t* exps;    /* powers of two of the scales' largest values, per row and per group */
     int64_t rows, cols;
     int64_t group_size;     /* columns per scale; >= cols: one scale per row */
 } llmc_int4_weight;
 
-/* Elements of packed, of scales (and zeros), and of exps.  group_size >= 16, or >= cols. */
-llmc_status llmc_int4_layout_sizes(int64_t rows, int64_t cols, int64_t group_size, int64_t* packed_words,
-                                   int64_t* entries, int64_t* exps);
+/* Bytes of packed and elements of exps.  group_size >= 16, or >= cols. */
+llmc_status llmc_int4_layout_sizes(int64_t rows, int64_t cols, int64_t group_size, int64_t* packed_bytes, int64_t* exps);
 /* Lays out one weight's codes as the GPTQ / RTN entry points write them for num_bits <= 4
  * ((q - zp) & 0xF, two per byte, even column high, crow bytes per row), with the scales and int32
  * zero-points (0..15; may be NULL when symmetric) of `strategy`, into w's arrays.  For TENSOR and

@@ -45,8 +45,6 @@ class Int4WeightC(C.Structure):
 
     _fields_ = [
         ("packed", C.c_void_p),
-        ("scales", C.c_void_p),
-        ("zeros", C.c_void_p),
         ("exps", C.c_void_p),
         ("rows", C.c_int64),
         ("cols", C.c_int64),
@@ -104,7 +102,7 @@ _SIGS = {
     "llmc_act_absmax": [P, P, I32, I64, I64, I64, P, I32],
     "llmc_smooth_apply": [P, P, P, I32, P, I32, I64, I64, F32, P],
     "llmc_scale_apply": [P, P, P, I32, P, I32, I64, I64],
-    "llmc_int4_layout_sizes": [I64, I64, I64, C.POINTER(I64), C.POINTER(I64), C.POINTER(I64)],
+    "llmc_int4_layout_sizes": [I64, I64, I64, C.POINTER(I64), C.POINTER(I64)],
     "llmc_int4_layout": [P, P, P, I64, P, P, I32, I32, P],
     "llmc_int4_dequantize": [P, P, P, I32, P, I64],
     "llmc_int4_linear_workspace": [P, P, P, I32, I64, I64, C.POINTER(I64)],

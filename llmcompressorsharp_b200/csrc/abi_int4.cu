@@ -21,7 +21,8 @@ struct DeviceScope {
 };
 
 constexpr int64_t MAX_DIM = (int64_t)1 << 30;     // rows, columns, tokens
-constexpr int64_t FEW = 16;                        // tokens that go to the few-row kernel
+// Tokens that go to the few-row kernel; it takes 16 at a time, and the codes anew for each 16.
+constexpr int64_t FEW_16 = 16, FEW_F32 = 128;
 
 llmc_status check_sizes(int64_t rows, int64_t cols, int64_t gs) {
     if (rows <= 0 || cols <= 0) return fail(LLMC_ERR_SHAPE, "a packed weight needs positive sizes (got %lld x %lld)", (long long)rows, (long long)cols);
@@ -33,12 +34,10 @@ llmc_status check_sizes(int64_t rows, int64_t cols, int64_t gs) {
 
 llmc_status view_of(const llmc_int4_weight* w, w4::View& v) {
     if (!w) return fail(LLMC_ERR_INVALID_ARG, "weight must not be null");
-    if (!w->packed || !w->scales || !w->zeros || !w->exps) return fail(LLMC_ERR_INVALID_ARG, "the weight's arrays must not be null");
+    if (!w->packed || !w->exps) return fail(LLMC_ERR_INVALID_ARG, "the weight's arrays must not be null");
     if ((uintptr_t)w->packed % 16 != 0) return fail(LLMC_ERR_INVALID_ARG, "packed must be 16-byte aligned");
     LLMC_TRY(check_sizes(w->rows, w->cols, w->group_size));
     v.packed = w->packed;
-    v.scales = w->scales;
-    v.zeros = w->zeros;
     v.exps = w->exps;
     w4::set_sizes(v, w->rows, w->cols, w->group_size);
     return LLMC_OK;
@@ -82,7 +81,7 @@ struct LinearPlan {
 LinearPlan plan_linear(const llmc_ctx* ctx, const w4::View& v, int dir, const void* a, int dtype, int64_t tokens, int64_t ld) {
     LinearPlan p{};
     const bool f32 = dtype == LLMC_DTYPE_F32;
-    p.few = dir == 0 && tokens <= FEW;
+    p.few = dir == 0 && tokens <= (f32 ? FEW_F32 : FEW_16);
     // 16-byte rows are what both kernels load; the few-row one reads whole vectors of eight columns, TMA
     // fills what is past the last column.  fp32 is read in bf16 pieces, other groups in the layout's columns.
     p.stage = f32 || (uintptr_t)a % 16 != 0 || (ld % 8 != 0) || (dir == 0 && !v.identity) || (p.few && v.cols % 8 != 0);
@@ -154,16 +153,14 @@ using namespace llmc;
 
 extern "C" {
 
-llmc_status llmc_int4_layout_sizes(int64_t rows, int64_t cols, int64_t group_size, int64_t* packed_words, int64_t* entries,
-                                   int64_t* exps) {
+llmc_status llmc_int4_layout_sizes(int64_t rows, int64_t cols, int64_t group_size, int64_t* packed_bytes, int64_t* exps) {
     LLMC_ENTRY();
-    if (!packed_words || !entries || !exps) return fail(LLMC_ERR_INVALID_ARG, "the sizes must not be null");
+    if (!packed_bytes || !exps) return fail(LLMC_ERR_INVALID_ARG, "the sizes must not be null");
     LLMC_TRY(check_sizes(rows, cols, group_size));
     w4::View v{};
     w4::set_sizes(v, rows, cols, group_size);
-    *packed_words = v.mp * (v.kp / 8);
-    *entries = v.mp * v.groups;
-    *exps = v.mp + v.groups;
+    *packed_bytes = v.mp / w4::ROWS * (v.kp / w4::TILE) * v.rec;
+    *exps = v.mp + v.kp / w4::TILE * v.ng;
     return LLMC_OK;
 }
 
@@ -186,8 +183,8 @@ llmc_status llmc_int4_layout(llmc_ctx* ctx, void* stream, const uint8_t* codes, 
         return fail(LLMC_ERR_SHAPE, "a tensor or channel scale needs group_size >= cols");
     DeviceScope scope;
     LLMC_TRY(scope.enter(ctx->device));
-    return int4_layout(ctx, stream_of(ctx, stream), codes, crow, scales, zps, srow, symmetric ? 1 : 0, v, const_cast<uint32_t*>(w->packed),
-                       const_cast<float*>(w->scales), const_cast<uint8_t*>(w->zeros), const_cast<int32_t*>(w->exps));
+    return int4_layout(ctx, stream_of(ctx, stream), codes, crow, scales, zps, srow, symmetric ? 1 : 0, v, const_cast<uint8_t*>(w->packed),
+                       const_cast<int32_t*>(w->exps));
 }
 
 llmc_status llmc_int4_dequantize(llmc_ctx* ctx, void* stream, const llmc_int4_weight* w, int32_t dtype, void* out, int64_t ldo) {

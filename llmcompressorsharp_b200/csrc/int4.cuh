@@ -8,29 +8,35 @@
 // row, leaves the columns where they were.  kp is their number rounded up to 128.  Rows are rounded
 // up to 128 (mp).  Codes that stand for no weight hold u = z, and rows past the last have s = 0.
 //
-// Tiles of 128 rows x 128 columns are 8 KB each, [row][64 bytes], the tiles of one row block one
-// after the other.  A row's 64 bytes are four 16-byte chunks t of four words c; word c of chunk t
-// holds columns 32 c + 8 t .. + 7, column 2 p in bits 4 p .. 4 p + 3 and column 2 p + 1 sixteen bits
-// above, so that (word >> 4 p) & 0x000F000F is a pair of neighbours.  A thread's 16-byte load then
-// is, for an m16n8k16 fragment, lane t's part of all four granules, and the pairs meet x unpermuted.
-// Scales and zeros are [group][mp]: the rows of a tile read them next to each other.
+// Tiles of 128 rows x 128 columns stand one row block after the other; a tile is eight records of 16 rows:
+//
+//   codes   16 rows x 64 bytes.  A row's 64 bytes are four 16-byte chunks t of four words c; word c of chunk t
+//           holds columns 32 c + 8 t .. + 7, column 2 p in bits 4 p .. 4 p + 3 and column 2 p + 1 sixteen bits
+//           above, so that (word >> 4 p) & 0x000F000F is a pair of neighbours.  A thread's 16-byte load then is,
+//           for an m16n8k16 fragment, lane t's part of all four granules, and the pairs meet x unpermuted.
+//   scales  16 rows x ng floats, ng = 1, 2 or 4 groups to a tile's 128 columns (the fewest that fit the group
+//           size; a group of 256 columns or more has its scale in each tile)
+//   zeros   16 rows x ng bytes
+//
+// So whatever a product needs for 16 rows x 128 columns is one stretch of 1,104 bytes (ng = 1), which one bulk
+// copy brings in, and nothing is fetched from a second place with a latency of its own.
 #pragma once
 #include "common.cuh"
 
 namespace llmc {
 namespace w4 {
 
-constexpr int TILE = 128;                 // rows and columns of a tile
-constexpr int TILE_WORDS = TILE * 16;     // 8 KB
+constexpr int TILE = 128;  // rows and columns of a tile
+constexpr int ROWS = 16;   // rows of a record
+constexpr int MAX_NG = 4;
 
 struct View {
-    const uint32_t* packed;
-    const float* scales;     // [groups][mp]
-    const uint8_t* zeros;    // [groups][mp]
-    const int32_t* exps;     // [mp] of the rows, then [groups]: see exps_kernel
+    const uint8_t* packed;
+    const int32_t* exps;     // [mp] of the rows, then [kp / 128 * ng] of the groups: see exps_kernel
     int64_t rows, cols;
     int64_t mp, kp;
     int32_t gs, gsv, groups;
+    int32_t ng, rec;         // groups per tile, bytes of a record
     int32_t identity;        // layout columns are the weight's own
 };
 
@@ -54,6 +60,8 @@ inline void set_sizes(View& v, int64_t rows, int64_t cols, int64_t gs) {
         v.kp = up((int64_t)(v.groups - 1) * v.gsv + (cols - (int64_t)(v.groups - 1) * gs), TILE);
         v.identity = gs % 32 == 0;
     }
+    v.ng = v.gsv % 128 == 0 ? 1 : v.gsv % 64 == 0 ? 2 : 4;
+    v.rec = 1024 + 80 * v.ng;
 }
 
 // Group of the granule that holds layout column kv (columns past the last group: the last).
@@ -61,6 +69,14 @@ __host__ __device__ __forceinline__ int group_of(int kv, int gsv, int groups) {
     const int g = kv / gsv;
     return g < groups ? g : groups - 1;
 }
+
+// Record of row r's 16 rows in the tile of columns 128 kt ..
+__host__ __device__ __forceinline__ int64_t record_at(const View& v, int64_t r, int64_t kt) {
+    return ((r / TILE * (v.kp / TILE) + kt) * (TILE / ROWS) + r % TILE / ROWS) * v.rec;
+}
+
+// Group, of a tile's ng, that granule c belongs to.
+__host__ __device__ __forceinline__ int slot_of(int c, int ng) { return c * ng / 4; }
 
 // The weight's column of layout column kv, -1 where none is.
 __host__ __device__ __forceinline__ int64_t column_of(int kv, int gs, int gsv, int groups, int64_t cols) {

@@ -5,6 +5,9 @@
 // they are: y[t][n] = sum_k x[t][k] (u - z) s + b[n].
 #include "int4.cuh"
 #include "ops.h"
+#include "tc_common.cuh"
+
+#include <atomic>
 
 namespace llmc {
 namespace {
@@ -20,9 +23,7 @@ struct LayoutArgs {
     int64_t srow;      // scale entries per row (0: one entry for the tensor)
     int sym;
     View v;
-    uint32_t* packed;
-    float* sout;
-    uint8_t* zout;
+    uint8_t* packed;
 };
 
 __device__ __forceinline__ uint32_t zero_of(const LayoutArgs& a, int64_t r, int g) {
@@ -30,17 +31,17 @@ __device__ __forceinline__ uint32_t zero_of(const LayoutArgs& a, int64_t r, int 
     return (uint32_t)a.zps[a.srow ? r * a.srow + g : 0] & 0xFu;
 }
 
-// One thread per word of eight codes; one read of the codes and one write, bound by memory.
+// One thread per word of eight codes, and per scale; one read of the codes and one write, bound by memory.
 __global__ void __launch_bounds__(256) layout_kernel(const LayoutArgs a) {
-    const int64_t words = a.v.mp * (a.v.kp / 8);
     const int64_t ktiles = a.v.kp / TILE;
+    const int64_t words = a.v.mp * (a.v.kp / 8);
     for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < words; i += (int64_t)gridDim.x * 256) {
-        const int64_t tile = i / TILE_WORDS;
-        const int in = (int)(i % TILE_WORDS), t = (in % 16) / 4, c = in % 4;
-        const int64_t r = tile / ktiles * TILE + in / 16;
+        const int64_t rec = i / (ROWS * 16);
+        const int in = (int)(i % (ROWS * 16)), t = in % 16 / 4, c = in % 4;
+        const int64_t tile = rec / (TILE / ROWS);
+        const int64_t r = tile / ktiles * TILE + rec % (TILE / ROWS) * ROWS + in / 16;
         const int kv0 = (int)(tile % ktiles) * TILE + 32 * c + 8 * t;
-        const int g = group_of(kv0, a.v.gsv, a.v.groups);
-        const uint32_t z = zero_of(a, r, g);
+        const uint32_t z = zero_of(a, r, group_of(kv0, a.v.gsv, a.v.groups));
         uint32_t w = 0;
 #pragma unroll
         for (int j = 0; j < 8; j++) {
@@ -54,30 +55,37 @@ __global__ void __launch_bounds__(256) layout_kernel(const LayoutArgs a) {
             }
             w |= u << ((j & 1) * 16 + (j >> 1) * 4);
         }
-        a.packed[i] = w;
+        *reinterpret_cast<uint32_t*>(a.packed + rec * a.v.rec + in * 4) = w;
     }
-    const int64_t entries = a.v.mp * a.v.groups;
+    const int64_t entries = a.v.mp * ktiles * a.v.ng;
     for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < entries; i += (int64_t)gridDim.x * 256) {
-        const int64_t g = i / a.v.mp, r = i % a.v.mp;
-        a.sout[i] = r < a.v.rows ? a.scales[a.srow ? r * a.srow + g : 0] : 0.f;
-        a.zout[i] = (uint8_t)zero_of(a, r, (int)g);
+        const int per = ROWS * a.v.ng;
+        const int64_t rec = i / per, tile = rec / (TILE / ROWS);
+        const int in = (int)(i % per), j = in % a.v.ng;
+        const int64_t r = tile / ktiles * TILE + rec % (TILE / ROWS) * ROWS + in / a.v.ng;
+        const int g = group_of((int)(tile % ktiles) * TILE + j * (TILE / a.v.ng), a.v.gsv, a.v.groups);
+        uint8_t* p = a.packed + rec * a.v.rec + 1024;
+        reinterpret_cast<float*>(p)[in] = r < a.v.rows ? a.scales[a.srow ? r * a.srow + g : 0] : 0.f;
+        p[64 * a.v.ng + in] = (uint8_t)zero_of(a, r, g);
     }
 }
 
-// Exponents that bring the scales near one before they meet fp16's range: for each row, and for each
-// group, e with 2^(e-1) <= max |s| < 2^e, within +-120 (0 where the maximum is 0 or not finite).  A product
+// Exponents that bring the scales near one before they meet fp16's range: for each row, and for each group of
+// each tile, e with 2^(e-1) <= max |s| < 2^e, within +-120 (0 where the maximum is 0 or not finite).  A product
 // kernel in fp16 uses s 2^-e and gives 2^e back in fp32, both exact.
-__global__ void __launch_bounds__(256) exps_kernel(const float* scales, int64_t mp, int groups, int32_t* exps) {
-    const int64_t row_blocks = mp / TILE;
+__global__ void __launch_bounds__(256) exps_kernel(const View v, int32_t* exps) {
+    const int64_t row_blocks = v.mp / TILE;
+    const int slots = (int)(v.kp / TILE) * v.ng;
+    const auto scale = [&](int64_t r, int s) {
+        return fabsf(reinterpret_cast<const float*>(v.packed + record_at(v, r, s / v.ng) + 1024)[r % ROWS * v.ng + s % v.ng]);
+    };
     float m = 0.f;
     __shared__ float sm[256];
     const bool rows = blockIdx.x < row_blocks;
     if (rows) {
-        const int64_t r = (int64_t)blockIdx.x * TILE + threadIdx.x % TILE;
-        for (int g = threadIdx.x / TILE; g < groups; g += 2) m = fmax_nan(m, fabsf(scales[(int64_t)g * mp + r]));
+        for (int s = threadIdx.x / TILE; s < slots; s += 2) m = fmax_nan(m, scale((int64_t)blockIdx.x * TILE + threadIdx.x % TILE, s));
     } else {
-        const int64_t g = blockIdx.x - row_blocks;
-        for (int64_t r = threadIdx.x; r < mp; r += 256) m = fmax_nan(m, fabsf(scales[g * mp + r]));
+        for (int64_t r = threadIdx.x; r < v.mp; r += 256) m = fmax_nan(m, scale(r, (int)(blockIdx.x - row_blocks)));
     }
     sm[threadIdx.x] = m;
     for (int step = 128; step >= (rows ? TILE : 1); step >>= 1) {
@@ -92,7 +100,7 @@ __global__ void __launch_bounds__(256) exps_kernel(const float* scales, int64_t 
     if (rows) {
         if (threadIdx.x < TILE) exps[(int64_t)blockIdx.x * TILE + threadIdx.x] = e;
     } else if (threadIdx.x == 0) {
-        exps[mp + blockIdx.x - row_blocks] = e;
+        exps[v.mp + blockIdx.x - row_blocks] = e;
     }
 }
 
@@ -132,12 +140,13 @@ __global__ void __launch_bounds__(256) rows_kernel(const View v, const I* ids, i
             if (!ok) atomicOr(flag, 1);
         }
         const int kv0 = b * 8;
-        const int g = group_of(kv0, v.gsv, v.groups);
         float val[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
         if (ok) {
-            const uint32_t w = v.packed[((r / TILE) * (v.kp / TILE) + kt) * TILE_WORDS + (r % TILE) * 16 + (kb % 4) * 4 + kb / 4];
-            const float s = v.scales[g * v.mp + r];
-            const int z = v.zeros[g * v.mp + r];
+            const uint8_t* rec = v.packed + record_at(v, r, kt);
+            const int in = (int)(r % ROWS), slot = in * v.ng + slot_of(kb / 4, v.ng);
+            const uint32_t w = reinterpret_cast<const uint32_t*>(rec)[in * 16 + (kb % 4) * 4 + kb / 4];
+            const float s = reinterpret_cast<const float*>(rec + 1024)[slot];
+            const int z = rec[1024 + 64 * v.ng + slot];
 #pragma unroll
             for (int j = 0; j < 8; j++) {
                 const int u = (int)(w >> ((j & 1) * 16 + (j >> 1) * 4)) & 0xF;
@@ -217,104 +226,191 @@ struct FewArgs {
     const void* bias;
     void* y;
     int64_t ldy;
+    int* err;
+    uint32_t wait_limit;
 };
+
+constexpr int RING = 4;       // steps in flight per warp
+constexpr int few_warps(int rb) { return 16 / rb; }  // per CTA at most
 
 // The codes are the A operand of m16n8k16 (16 weight rows x 16 columns), x the B operand (8 tokens), so one
 // dequantised fragment serves eight tokens and a single token costs no more than the codes.  Codes enter as
-// the exact integers u - z; the fp32 sum of a group is multiplied by its scale (FL granules of 32 columns
-// per group sum), so x and W are never rounded.
-// A CTA holds 16 rows; its warps take the 128-column tiles in turn and add their sums in shared memory, in
-// warp order.
-template <typename T, typename O, int NT, int PIECES, int FL>
-__global__ void __launch_bounds__(256) few_kernel(const FewArgs a) {
-    extern __shared__ float red[];  // [warps][16][8 NT]
+// the exact integers u - z; the fp32 sum of a group is multiplied by its scale (4 / NG granules of 32 columns per
+// group sum), so x and W are never rounded.
+// A CTA holds RB records' rows (16 RB) and 8 NT tokens at a time; its warps take the 128-column steps in turn, each
+// through a ring of its own that bulk copies keep full across rows, and add their sums in shared memory, in warp order.
+template <typename T, typename O, int NT, int PIECES, int NG, int RB>
+__global__ void __launch_bounds__(32 * few_warps(RB)) few_kernel(const FewArgs a) {
+    constexpr int REC = 1024 + 80 * NG, STEP = RB * REC, FL = 4 / NG, SUMS = 8 * NT * ROWS * RB;
+    extern __shared__ __align__(128) uint8_t smem[];  // rings, barriers, two [warps][8 NT][16 RB] of sums
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, warps = blockDim.x / 32;
+    uint8_t* ring = smem + warp * RING * STEP;
+    uint64_t* bars = reinterpret_cast<uint64_t*>(smem + warps * RING * STEP) + warp * RING;
+    float* red = reinterpret_cast<float*>(smem + warps * RING * (STEP + 8));
     const int g = lane >> 2, t = lane & 3;
-    const int64_t row0 = (int64_t)blockIdx.x * 16;
     const int ktiles = (int)(a.v.kp / TILE);
-    const uint4* wp = reinterpret_cast<const uint4*>(a.v.packed) + (row0 / TILE) * ktiles * (TILE_WORDS / 4) +
-                      (row0 % TILE + g) * 4 + t;
-    const T* x = reinterpret_cast<const T*>(a.x);
-    float acc[NT][4];
+    const int blocks = (int)((a.v.rows + ROWS * RB - 1) / (ROWS * RB));
+    const int tok0 = blockIdx.y * 8 * NT;
+    if (lane == 0) {
+        for (int s = 0; s < RING; s++) tc::mbar_init(&bars[s], 1);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    __syncwarp();
+
+    // the next step to fetch: row block prb, tile pkt, in the ring's stage pst
+    int prb = blockIdx.x, pkt = warp, pst = 0;
+    uint32_t fetched = 0, used = 0;
+    bool failed = false;
+    const uint8_t* src = a.v.packed + record_at(a.v, (int64_t)prb * (ROWS * RB), pkt);
+    const int64_t hop = (int64_t)warps * (TILE / ROWS) * REC;
+    auto fetch = [&]() {
+        if (prb >= blocks || failed) return;
+        if (lane == 0) {
+            tc::mbar_expect_tx(&bars[pst], STEP);
+            tc::bulk_load(ring + pst * STEP, src, STEP, &bars[pst]);
+        }
+        fetched++;
+        pst = pst == RING - 1 ? 0 : pst + 1;
+        pkt += warps;
+        src += hop;
+        if (pkt >= ktiles) {
+            pkt = warp;
+            prb += gridDim.x;
+            src = a.v.packed + record_at(a.v, (int64_t)prb * (ROWS * RB), pkt);
+        }
+    };
+    for (int s = 0; s < RING; s++) fetch();
+
+    // this lane's token of each eight and piece, at its columns of the first granule
+    const T* xp[NT][PIECES];
 #pragma unroll
     for (int n = 0; n < NT; n++)
 #pragma unroll
-        for (int j = 0; j < 4; j++) acc[n][j] = 0.f;
-
-    uint4 wa, wb;
-    if (warp < ktiles) {
-        wa = __ldcs(wp + (int64_t)warp * (TILE_WORDS / 4));
-        wb = __ldcs(wp + (int64_t)warp * (TILE_WORDS / 4) + 8 * 4);
-    }
-    for (int kt = warp; kt < ktiles; kt += warps) {
-        const uint4 ca = wa, cb = wb;
-        if (kt + warps < ktiles) {
-            wa = __ldcs(wp + (int64_t)(kt + warps) * (TILE_WORDS / 4));
-            wb = __ldcs(wp + (int64_t)(kt + warps) * (TILE_WORDS / 4) + 8 * 4);
+        for (int p = 0; p < PIECES; p++) {
+            const int tok = tok0 + n * 8 + g;
+            xp[n][p] = tok < a.tokens ? reinterpret_cast<const T*>(a.x) + ((int64_t)p * a.tokens + tok) * a.ldx + 8 * t : nullptr;
         }
-        const uint32_t w0[4] = {ca.x, ca.y, ca.z, ca.w}, w1[4] = {cb.x, cb.y, cb.z, cb.w};
-        float d[NT][4];
-        uint32_t z0 = 0, z1 = 0;
-        float s0 = 0.f, s1 = 0.f;
+    auto load_x = [&](int kt, uint4 (&b)[4][NT][PIECES]) {
 #pragma unroll
-        for (int c = 0; c < 4; c++) {
-            const int kv = kt * TILE + 32 * c;
-            if (c % FL == 0) {
-                const int64_t o = (int64_t)group_of(kv, a.v.gsv, a.v.groups) * a.v.mp + row0 + g;
-                s0 = a.v.scales[o];
-                s1 = a.v.scales[o + 8];
-                z0 = zero_pair<T>(a.v.zeros[o]);
-                z1 = zero_pair<T>(a.v.zeros[o + 8]);
+        for (int c = 0; c < 4; c++)
 #pragma unroll
-                for (int n = 0; n < NT; n++)
+            for (int n = 0; n < NT; n++)
 #pragma unroll
-                    for (int j = 0; j < 4; j++) d[n][j] = 0.f;
+                for (int p = 0; p < PIECES; p++) {
+                    const int k = kt * TILE + 32 * c;
+                    b[c][n][p] = make_uint4(0, 0, 0, 0);
+                    if (xp[n][p] && k + 8 * t < a.xcols) b[c][n][p] = __ldg(reinterpret_cast<const uint4*>(xp[n][p] + k));
+                }
+    };
+    constexpr bool AHEAD = NT * PIECES <= 2;  // 16 registers for each of NT and PIECES
+    uint4 nb[4][NT][PIECES];
+    if constexpr (AHEAD) load_x(warp, nb);
+    int flip = 0, st = 0;
+    for (int rb = blockIdx.x; rb < blocks; rb += gridDim.x, flip ^= 1) {
+        float acc[RB][NT][4];
+#pragma unroll
+        for (int r = 0; r < RB; r++)
+#pragma unroll
+            for (int n = 0; n < NT; n++)
+#pragma unroll
+                for (int j = 0; j < 4; j++) acc[r][n][j] = 0.f;
+        for (int kt = warp; kt < ktiles && !failed; kt += warps) {
+            uint4 b[4][NT][PIECES];
+            if constexpr (AHEAD) {
+                // the next step's x while this one is multiplied: with one row block to a CTA each of these is a miss of L1
+#pragma unroll
+                for (int c = 0; c < 4; c++)
+#pragma unroll
+                    for (int n = 0; n < NT; n++)
+#pragma unroll
+                        for (int p = 0; p < PIECES; p++) b[c][n][p] = nb[c][n][p];
+                load_x(kt + warps < ktiles ? kt + warps : warp, nb);
+            } else {
+                load_x(kt, b);
             }
-            const uint32_t f0[4] = {int_pair<T>(w0[c], 0, z0), int_pair<T>(w1[c], 0, z1), int_pair<T>(w0[c], 1, z0),
-                                    int_pair<T>(w1[c], 1, z1)};
-            const uint32_t f1[4] = {int_pair<T>(w0[c], 2, z0), int_pair<T>(w1[c], 2, z1), int_pair<T>(w0[c], 3, z0),
-                                    int_pair<T>(w1[c], 3, z1)};
-            const int k = kv + 8 * t;
+            if (!tc::mbar_wait_bounded(&bars[st], (used / RING) & 1u, a.wait_limit)) failed = true;
+            if (__any_sync(0xffffffffu, failed)) {
+                failed = true;
+                break;
+            }
+            used++;
+            const uint8_t* rec = ring + st * STEP;
+            st = st == RING - 1 ? 0 : st + 1;
+            uint32_t w[RB][2][4], zz[RB][2][NG];
+            float sc[RB][2][NG];
 #pragma unroll
-            for (int n = 0; n < NT; n++) {
-                const int tok = n * 8 + g;
+            for (int r = 0; r < RB; r++)
 #pragma unroll
-                for (int p = PIECES - 1; p >= 0; p--) {
-                    uint4 b = make_uint4(0, 0, 0, 0);
-                    if (tok < a.tokens && k < a.xcols)
-                        b = __ldg(reinterpret_cast<const uint4*>(x + ((int64_t)p * a.tokens + tok) * a.ldx + k));
-                    mma16816(d[n], f0, b.x, b.y, T());
-                    mma16816(d[n], f1, b.z, b.w, T());
+                for (int i = 0; i < 2; i++) {
+                    const int row = g + 8 * i;
+                    const uint8_t* q = rec + r * REC;
+                    const uint4 u = *reinterpret_cast<const uint4*>(q + row * 64 + t * 16);
+                    w[r][i][0] = u.x;
+                    w[r][i][1] = u.y;
+                    w[r][i][2] = u.z;
+                    w[r][i][3] = u.w;
+#pragma unroll
+                    for (int j = 0; j < NG; j++) {
+                        sc[r][i][j] = reinterpret_cast<const float*>(q + 1024)[row * NG + j];
+                        zz[r][i][j] = zero_pair<T>(q[1024 + 64 * NG + row * NG + j]);
+                    }
+                }
+            __syncwarp();
+            fetch();  // into the stage just read
+            float d[RB][NT][4];
+#pragma unroll
+            for (int c = 0; c < 4; c++) {
+                const int j = c / FL;
+#pragma unroll
+                for (int r = 0; r < RB; r++) {
+                    if (c % FL == 0)
+#pragma unroll
+                        for (int n = 0; n < NT; n++)
+#pragma unroll
+                            for (int i = 0; i < 4; i++) d[r][n][i] = 0.f;
+                    uint32_t f[2][4];
+#pragma unroll
+                    for (int h = 0; h < 2; h++)
+#pragma unroll
+                        for (int i = 0; i < 4; i++) f[h][i] = int_pair<T>(w[r][i & 1][c], 2 * h + i / 2, zz[r][i & 1][j]);
+#pragma unroll
+                    for (int n = 0; n < NT; n++)
+#pragma unroll
+                        for (int p = PIECES - 1; p >= 0; p--) {
+                            mma16816(d[r][n], f[0], b[c][n][p].x, b[c][n][p].y, T());
+                            mma16816(d[r][n], f[1], b[c][n][p].z, b[c][n][p].w, T());
+                        }
+                    if (c % FL == FL - 1)
+#pragma unroll
+                        for (int n = 0; n < NT; n++)
+#pragma unroll
+                            for (int i = 0; i < 4; i++) acc[r][n][i] = fmaf(sc[r][i / 2][j], d[r][n][i], acc[r][n][i]);
                 }
             }
-            if (c % FL == FL - 1) {
+        }
+        float* sums = red + flip * warps * SUMS;
 #pragma unroll
-                for (int n = 0; n < NT; n++) {
-                    acc[n][0] = fmaf(s0, d[n][0], acc[n][0]);
-                    acc[n][1] = fmaf(s0, d[n][1], acc[n][1]);
-                    acc[n][2] = fmaf(s1, d[n][2], acc[n][2]);
-                    acc[n][3] = fmaf(s1, d[n][3], acc[n][3]);
-                }
-            }
+        for (int r = 0; r < RB; r++)
+#pragma unroll
+            for (int n = 0; n < NT; n++)
+#pragma unroll
+                for (int i = 0; i < 4; i++)  // [warp][token][row]
+                    sums[warp * SUMS + (n * 8 + 2 * t + (i & 1)) * (ROWS * RB) + r * ROWS + g + 8 * (i / 2)] = acc[r][n][i];
+        __syncthreads();  // the other buffer's readers have all passed the sync before this one
+        for (int i = threadIdx.x; i < SUMS; i += blockDim.x) {
+            const int64_t row = (int64_t)rb * (ROWS * RB) + i % (ROWS * RB);
+            const int tok = tok0 + i / (ROWS * RB);
+            if (row >= a.v.rows || tok >= a.tokens) continue;
+            float s = 0.f;
+            for (int w = 0; w < warps; w++) s += sums[w * SUMS + i];
+            if (a.bias) s += to_f<O>(reinterpret_cast<const O*>(a.bias)[row]);
+            reinterpret_cast<O*>(a.y)[tok * a.ldy + row] = from_f<O>(s);
         }
     }
-#pragma unroll
-    for (int n = 0; n < NT; n++) {
-        float* r = red + (warp * 8 * NT + n * 8 + 2 * t) * 16 + g;  // [warp][token][row]
-        r[0] = acc[n][0];
-        r[16] = acc[n][1];
-        r[8] = acc[n][2];
-        r[24] = acc[n][3];
-    }
-    __syncthreads();
-    for (int i = threadIdx.x; i < 16 * 8 * NT; i += blockDim.x) {
-        const int64_t row = row0 + i % 16;
-        const int tok = i / 16;
-        if (row >= a.v.rows || tok >= a.tokens) continue;
-        float s = 0.f;
-        for (int w = 0; w < warps; w++) s += red[w * 8 * NT * 16 + i];
-        if (a.bias) s += to_f<O>(reinterpret_cast<const O*>(a.bias)[row]);
-        reinterpret_cast<O*>(a.y)[tok * a.ldy + row] = from_f<O>(s);
+    // after a wait that gave up, copies may still be on their way
+    if (failed) {
+        atomicOr(a.err, 1);
+        for (; used < fetched; used++) tc::mbar_wait_drain(&bars[used % RING], (used / RING) & 1u);
     }
 }
 
@@ -357,25 +453,64 @@ int grid_n(const llmc_ctx* ctx, int64_t items) {
     return (int)(b < 1 ? 1 : (b > cap ? cap : b));
 }
 
-template <typename T, typename O, int NT, int PIECES>
-void launch_few(const FewArgs& a, int warps, cudaStream_t st) {
-    const unsigned grid = (unsigned)((a.v.rows + 15) / 16);
-    const size_t sm = (size_t)warps * 16 * 8 * NT * sizeof(float);
-    // granules per group sum: the largest of 4, 2, 1 that divides the group
-    if (a.v.gsv % 128 == 0) few_kernel<T, O, NT, PIECES, 4><<<grid, warps * 32, sm, st>>>(a);
-    else if (a.v.gsv % 64 == 0) few_kernel<T, O, NT, PIECES, 2><<<grid, warps * 32, sm, st>>>(a);
-    else few_kernel<T, O, NT, PIECES, 1><<<grid, warps * 32, sm, st>>>(a);
+// CTAs of `threads` that an SM holds; asked once per kernel and number of warps.
+template <auto kernel> int resident(int device, int warps, size_t smem) {
+    static std::atomic<int> known[64][few_warps(1) + 1];
+    if (device < 0 || device >= 64) return 1;
+    int n = known[device][warps].load(std::memory_order_relaxed);
+    if (n == 0) {
+        if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024) != cudaSuccess ||
+            cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kernel, warps * 32, smem) != cudaSuccess || n < 1) {
+            cudaGetLastError();
+            return 0;
+        }
+        known[device][warps].store(n, std::memory_order_relaxed);
+    }
+    return n;
+}
+
+template <typename T, typename O, int NT, int PIECES, int NG, int RB>
+llmc_status launch_few(llmc_ctx* ctx, const FewArgs& a, cudaStream_t st) {
+    constexpr int STEP = RB * (1024 + 80 * NG);
+    const int64_t blocks = (a.v.rows + ROWS * RB - 1) / (ROWS * RB);
+    const int ktiles = (int)(a.v.kp / TILE), tiles = (a.tokens + 8 * NT - 1) / (8 * NT);
+    // sixteen warps to a CTA where the rows give an SM two CTAs or fewer, eight where they give more: see few_kernel
+    const int most = blocks * tiles <= 2 * ctx->sm_count ? few_warps(RB) : 8;
+    const int warps = ktiles < most ? ktiles : most;
+    constexpr int SUMS = 2 * 8 * NT * ROWS * RB * (int)sizeof(float);
+    static_assert(few_warps(RB) * (RING * (STEP + 8) + SUMS) <= 227 * 1024, "shared memory of an SM");
+    const size_t sm = (size_t)warps * (RING * (STEP + 8) + SUMS);
+    constexpr auto kernel = few_kernel<T, O, NT, PIECES, NG, RB>;
+    const int per = resident<kernel>(ctx->device, warps, sm);
+    if (per < 1) return fail(LLMC_ERR_CUDA, "the packed product's kernel does not fit this device");
+    int64_t cap = (int64_t)per * persistent_sms(ctx) / tiles;
+    if (cap < 1) cap = 1;
+    kernel<<<dim3((unsigned)(blocks < cap ? blocks : cap), (unsigned)tiles), warps * 32, sm, st>>>(a);
+    return check_launch(ctx, "int4_few");
+}
+
+template <typename T, typename O, int NT, int PIECES, int RB>
+llmc_status few_by_group(llmc_ctx* ctx, const FewArgs& a, cudaStream_t st) {
+    if (a.v.ng == 1) return launch_few<T, O, NT, PIECES, 1, RB>(ctx, a, st);
+    if (a.v.ng == 2) return launch_few<T, O, NT, PIECES, 2, RB>(ctx, a, st);
+    return launch_few<T, O, NT, PIECES, 4, RB>(ctx, a, st);
+}
+
+template <typename T, typename O, int PIECES> llmc_status few_by_size(llmc_ctx* ctx, const FewArgs& a, cudaStream_t st) {
+    // Two records a step share the loads of x (NT PIECES x 2 KB a step from L1, against 1 KB of codes a record); with few
+    // rows one, which makes twice the CTAs.
+    if (a.tokens > 8) return few_by_group<T, O, 2, PIECES, 2>(ctx, a, st);
+    return few_by_group<T, O, 1, PIECES, 1>(ctx, a, st);
 }
 
 }  // namespace
 
 llmc_status int4_layout(llmc_ctx* ctx, cudaStream_t st, const uint8_t* codes, int64_t crow, const float* scales,
-                        const int32_t* zps, int64_t srow, int sym, const w4::View& v, uint32_t* packed, float* sout,
-                        uint8_t* zout, int32_t* exps) {
-    LayoutArgs a{codes, crow, scales, zps, srow, sym, v, packed, sout, zout};
+                        const int32_t* zps, int64_t srow, int sym, const w4::View& v, uint8_t* packed, int32_t* exps) {
+    LayoutArgs a{codes, crow, scales, zps, srow, sym, v, packed};
     layout_kernel<<<grid_n(ctx, v.mp * (v.kp / 8)), 256, 0, st>>>(a);
     LLMC_TRY(check_launch(ctx, "int4_layout"));
-    exps_kernel<<<(unsigned)(v.mp / TILE + v.groups), 256, 0, st>>>(sout, v.mp, v.groups, exps);
+    exps_kernel<<<(unsigned)(v.mp / TILE + v.kp / TILE * v.ng), 256, 0, st>>>(v, exps);
     return check_launch(ctx, "int4_exps");
 }
 
@@ -412,21 +547,10 @@ llmc_status int4_stage(llmc_ctx* ctx, cudaStream_t st, const void* x, int dtype,
 
 llmc_status int4_few(llmc_ctx* ctx, cudaStream_t st, const w4::View& v, const void* x, int dtype, int64_t tokens, int64_t ldx,
                      int64_t xcols, const void* bias, void* y, int64_t ldy) {
-    FewArgs a{v, x, ldx, xcols, (int)tokens, bias, y, ldy};
-    const int ktiles = (int)(v.kp / TILE);
-    const int warps = ktiles < 8 ? ktiles : 8;
-    const bool two = tokens > 8;
-    if (dtype == LLMC_DTYPE_F32) {
-        if (two) launch_few<__nv_bfloat16, float, 2, 3>(a, warps, st);
-        else launch_few<__nv_bfloat16, float, 1, 3>(a, warps, st);
-    } else if (dtype == LLMC_DTYPE_BF16) {
-        if (two) launch_few<__nv_bfloat16, __nv_bfloat16, 2, 1>(a, warps, st);
-        else launch_few<__nv_bfloat16, __nv_bfloat16, 1, 1>(a, warps, st);
-    } else {
-        if (two) launch_few<__half, __half, 2, 1>(a, warps, st);
-        else launch_few<__half, __half, 1, 1>(a, warps, st);
-    }
-    return check_launch(ctx, "int4_few");
+    FewArgs a{v, x, ldx, xcols, (int)tokens, bias, y, ldy, ctx->dflags + 2, ctx->wait_limit};
+    if (dtype == LLMC_DTYPE_F32) return few_by_size<__nv_bfloat16, float, 3>(ctx, a, st);
+    if (dtype == LLMC_DTYPE_BF16) return few_by_size<__nv_bfloat16, __nv_bfloat16, 1>(ctx, a, st);
+    return few_by_size<__half, __half, 1>(ctx, a, st);
 }
 
 llmc_status int4_join(llmc_ctx* ctx, cudaStream_t st, const float* part, int splits, int64_t rows, int64_t cols, const void* bias,

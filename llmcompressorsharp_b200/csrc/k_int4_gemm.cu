@@ -21,8 +21,12 @@
 // to fp32 registers.
 //
 // A persistent grid of CTA pairs (256 tokens x 256 columns, cta_group::2) or, for up to 128 tokens and for fp32,
-// single CTAs (128 x 128).  Per CTA: a TMA warp, an MMA warp, epilogue warps, eight dequantising warps, a ring of
-// STAGES x (16 KB activations + 16 KB weights), two accumulators in TMEM.  Every wait is bounded.
+// single CTAs (128 x 128).  Per CTA: a TMA warp for the activations and one for the codes (a tile of eight records,
+// 128 x 128 weights, in one bulk copy), an MMA warp, epilogue warps, eight dequantising warps, a ring of
+// STAGES x (32 KB activations + 32 KB weights) and one of CODE_STAGES tiles of codes, two accumulators in TMEM.
+// A stage is a whole tile, 128 of the contraction: the MMA thread's two waits and its commit take about 700 clocks,
+// which a stage of 64 (512 clocks of MMAs) did not cover (0.59 us a stage; see the figures at int4_gemm).
+// Every wait is bounded.
 #include "int4.cuh"
 #include "ops.h"
 #include "tc_common.cuh"
@@ -37,17 +41,20 @@ namespace {
 using namespace tc;
 using namespace w4;
 
-constexpr int BK = 64, STAGES = 6;
-constexpr int A_BYTES = 128 * BK * 2, B_BYTES = 128 * BK * 2, STAGE_BYTES = A_BYTES + B_BYTES;
-constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + 1024 + 256;
+constexpr int BOX = 64;                       // columns of a TMA box: 128 bytes, the swizzle's width
+constexpr int BOX_BYTES = 128 * BOX * 2;
+constexpr int STAGES = 3, A_BYTES = 2 * BOX_BYTES, B_BYTES = 2 * BOX_BYTES, STAGE_BYTES = A_BYTES + B_BYTES;
+constexpr int CODE_STAGES = 3, CODE_BYTES = (TILE / ROWS) * (1024 + 80 * MAX_NG);  // tiles of codes
+constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + CODE_STAGES * CODE_BYTES + 1024 + 256;
+static_assert(SMEM_BYTES <= 227 * 1024, "shared memory of a CTA");
 constexpr int DQ_WARPS = 8;
-constexpr int FOLD_KB = 4;  // k-blocks between folds (fp32)
+constexpr int FOLD = 2;  // tiles of the contraction between folds (fp32)
 
 struct GemmInt4 {
     View v;
     int64_t tokens;
     int64_t ocols;           // columns of the output
-    int tiles_m, tiles_n, splits, kb_total, kb_per, group_m;
+    int tiles_m, tiles_n, splits, kt_total, kt_per, group_m;  // kt: tiles of 128 of the contraction, one stage each
     int64_t piece_rows;      // rows between the pieces of the activations' map
     const void* bias;
     void* out;
@@ -61,7 +68,7 @@ struct GemmInt4 {
 
 struct Unit {
     int64_t m0, n0;  // first token and column of the tile
-    int kb0, kb1, split;
+    int kt0, kt1, split;
 };
 
 template <int CG> __device__ __forceinline__ Unit unit_at(const GemmInt4& a, int u) {
@@ -73,8 +80,8 @@ template <int CG> __device__ __forceinline__ Unit unit_at(const GemmInt4& a, int
     const int per = a.group_m * a.tiles_n, g = t / per, first = g * a.group_m, gm = min(a.group_m, a.tiles_m - first), l = t - g * per;
     r.m0 = (int64_t)(first + l % gm) * (128 * CG);
     r.n0 = (int64_t)(l / gm) * (128 * CG);
-    r.kb0 = r.split * a.kb_per;
-    r.kb1 = min(a.kb_total, r.kb0 + a.kb_per);
+    r.kt0 = r.split * a.kt_per;
+    r.kt1 = min(a.kt_total, r.kt0 + a.kt_per);
     return r;
 }
 
@@ -85,120 +92,48 @@ __device__ __forceinline__ void combo(int c, int& xp, int& wp) {
     wp = c == 1 ? 2 : (c == 2 || c == 4) ? 1 : 0;
 }
 
-// One stage's codes of one thread with their scales: forward, 64 columns of one row (granules 2); gradient, 64
-// columns (chunks 2 hh, 2 hh + 1) of one row (granules 4).
-struct Frag {
-    uint32_t w[8];
-    float s[4];
-    uint8_t z[4];
-};
+// Two groups of four dequantising warps take the tiles in turn, so that one converts while the other waits, fences or
+// signals; a warp has two records of a tile, four rows' chunks (sixteen words) to a thread.
+// Lanes 4 i .. 4 i + 3 hold the chunks of one row, in the order of rows below: an 8-lane phase then meets
+// rows of different parity, so that its 16-byte loads (rows 64 bytes apart) touch every bank once, and of
+// different bit 2, so that its stores into the 128-byte swizzle do.
+__device__ __forceinline__ int row_of(int lane) { return (0x36271450 >> (lane / 4 * 4)) & 7; }
 
-template <int DIR>
-__device__ __forceinline__ void load_frag(const View& v, int64_t n0, int kb, int tid, Frag& f) {
-    if constexpr (DIR == 0) {
-        const int64_t n = n0 + tid;
-        const int kt = kb >> 1, h = kb & 1;
-        const uint2* p = reinterpret_cast<const uint2*>(v.packed + ((n / TILE) * (v.kp / TILE) + kt) * TILE_WORDS + (n % TILE) * 16 + 2 * h);
-#pragma unroll
-        for (int t = 0; t < 4; t++) {
-            const uint2 q = __ldg(p + 2 * t);
-            f.w[2 * t] = q.x;
-            f.w[2 * t + 1] = q.y;
-        }
-#pragma unroll
-        for (int c = 0; c < 2; c++) {
-            if (c && v.gsv % 64 == 0) {
-                f.s[1] = f.s[0];
-                f.z[1] = f.z[0];
-                break;
-            }
-            const int64_t o = (int64_t)group_of(kb * BK + 32 * c, v.gsv, v.groups) * v.mp + n;
-            f.s[c] = __ldg(v.scales + o);
-            f.z[c] = __ldg(v.zeros + o);
-        }
-    } else {
-        const int64_t n = (int64_t)kb * BK + tid % 64;
-        const int hh = tid / 64;
-        const uint4* p = reinterpret_cast<const uint4*>(v.packed + ((n / TILE) * (v.kp / TILE) + n0 / TILE) * TILE_WORDS + (n % TILE) * 16) + 2 * hh;
-#pragma unroll
-        for (int q = 0; q < 2; q++) {
-            const uint4 x = __ldg(p + q);
-            f.w[4 * q] = x.x;
-            f.w[4 * q + 1] = x.y;
-            f.w[4 * q + 2] = x.z;
-            f.w[4 * q + 3] = x.w;
-        }
-#pragma unroll
-        for (int c = 0; c < 4; c++) {
-            if (c && v.gsv % 128 == 0) {
-                f.s[c] = f.s[0];
-                f.z[c] = f.z[0];
-                continue;
-            }
-            const int64_t o = (int64_t)group_of((int)n0 + 32 * c, v.gsv, v.groups) * v.mp + n;
-            f.s[c] = __ldg(v.scales + o);
-            f.z[c] = __ldg(v.zeros + o);
+// A scale and zero ready for eight weights at a time.
+template <typename T, int PIECES> struct Scale {
+    typename Num<T>::T2 hi, lo;  // PIECES == 1
+    float s;
+    uint32_t zz;
+    __device__ __forceinline__ void set(float scale, uint32_t z) {
+        zz = zero_pair<T>(z);
+        s = scale;
+        if constexpr (PIECES == 1) {
+            hi.x = hi.y = from_f<T>(scale);
+            lo.x = lo.y = from_f<T>(__fsub_rn(scale, to_f<T>(hi.x)));
         }
     }
-}
+};
 
-// Eight weights of a word in T: rounded once, or piece wp of their fp32 value.
+// Eight weights of a word in T: rounded once, or piece wp of their fp32 value (truncated, eight bits each, so the three
+// add up to it).
 template <typename T, int PIECES>
-__device__ __forceinline__ uint4 dequant(uint32_t word, float s, uint32_t z, int wp) {
+__device__ __forceinline__ uint4 dequant(uint32_t word, const Scale<T, PIECES>& sc, int wp) {
     uint32_t o[4];
-    const uint32_t zz = zero_pair<T>(z);
-    if constexpr (PIECES == 1) {
-        const T hi = from_f<T>(s);
-        const T lo = from_f<T>(__fsub_rn(s, to_f<T>(hi)));
-        typename Num<T>::T2 hi2, lo2;
-        hi2.x = hi2.y = hi;
-        lo2.x = lo2.y = lo;
 #pragma unroll
-        for (int p = 0; p < 4; p++) {
-            const auto v = as2<T>(int_pair<T>(word, p, zz));
-            o[p] = bits2(__hfma2(v, hi2, __hmul2(v, lo2)));
-        }
-    } else {
-#pragma unroll
-        for (int p = 0; p < 4; p++) {
-            const uint32_t v = int_pair<T>(word, p, zz);
-            uint32_t r = 0;
-#pragma unroll
-            for (int j = 0; j < 2; j++) {
-                const float i = __uint_as_float(j ? (v & 0xFFFF0000u) : (v << 16));
-                float w = __fmul_rn(i, s);
-                __nv_bfloat16 b = __float2bfloat16_rn(w);
-                for (int q = 0; q < wp; q++) {
-                    w = __fsub_rn(w, __bfloat162float(b));
-                    b = __float2bfloat16_rn(w);
-                }
-                r |= (uint32_t)__bfloat16_as_ushort(b) << (16 * j);
+    for (int p = 0; p < 4; p++) {
+        const uint32_t v = int_pair<T>(word, p, sc.zz);
+        if constexpr (PIECES == 1) {
+            o[p] = bits2(__hfma2(as2<T>(v), sc.hi, __hmul2(as2<T>(v), sc.lo)));
+        } else {
+            float w0 = __fmul_rn(__uint_as_float(v << 16), sc.s), w1 = __fmul_rn(__uint_as_float(v & 0xFFFF0000u), sc.s);
+            for (int q = 0; q < wp; q++) {
+                w0 = __fsub_rn(w0, __uint_as_float(__float_as_uint(w0) & 0xFFFF0000u));
+                w1 = __fsub_rn(w1, __uint_as_float(__float_as_uint(w1) & 0xFFFF0000u));
             }
-            o[p] = r;
+            o[p] = __byte_perm(__float_as_uint(w0), __float_as_uint(w1), 0x7632);
         }
     }
     return make_uint4(o[0], o[1], o[2], o[3]);
-}
-
-template <typename T, int DIR, int PIECES>
-__device__ __forceinline__ void store_frag(const Frag& f, unsigned char* b, int tid, int wp, const int* e) {
-#pragma unroll
-    for (int i = 0; i < 8; i++) {
-        int c, off;
-        if constexpr (DIR == 0) {
-            const int t = i / 2;
-            c = i % 2;
-            off = tid * 128 + (((4 * c + t) ^ (tid & 7)) << 4);
-        } else {
-            const int t = 2 * (tid / 64) + i / 4, r = tid % 64;
-            c = i % 4;
-            off = (c / 2) * (64 * BK * 2) + r * 128 + (((4 * (c & 1) + t) ^ (r & 7)) << 4);
-        }
-        float s = f.s[c];
-        if constexpr (sizeof(T) == 2 && PIECES == 1)
-            if (Num<T>::MAGIC == Num<__half>::MAGIC) s *= pow2(-e[DIR == 0 ? 0 : c]);
-        *reinterpret_cast<uint4*>(b + off) = dequant<T, PIECES>(f.w[i], s, f.z[c], wp);
-    }
 }
 
 template <int CG> __device__ __forceinline__ void commit(uint64_t* bar) {
@@ -208,21 +143,24 @@ template <int CG> __device__ __forceinline__ void commit(uint64_t* bar) {
 
 // T: operand type; O: output (and bias) type; DIR 0 forward, 1 gradient; CG CTAs per tile; PIECES 1, or 3 for fp32.
 template <typename T, typename O, int DIR, int CG, int PIECES>
-__global__ void __launch_bounds__(32 * (2 + (PIECES == 3 ? 8 : 4) + DQ_WARPS), 1)
+__global__ void __launch_bounds__(32 * (3 + (PIECES == 3 ? 8 : 4) + DQ_WARPS), 1)
     gemm_int4_kernel(const __grid_constant__ CUtensorMap amap, const __grid_constant__ GemmInt4 a) {
-    constexpr bool FOLD = PIECES == 3;
-    constexpr int EW = FOLD ? 8 : 4;          // epilogue warps
+    constexpr bool FOLDS = PIECES == 3;
+    constexpr int EW = FOLDS ? 8 : 4;          // epilogue warps
     constexpr int BN = 128 * CG;              // columns of a tile
     constexpr int TMEM_COLS = 2 * BN;
     constexpr int EC = BN * 4 / EW;           // columns per epilogue warp
     extern __shared__ unsigned char smem_raw[];
     unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-    uint64_t* afull = reinterpret_cast<uint64_t*>(smem + STAGES * STAGE_BYTES);
+    unsigned char* codes = smem + STAGES * STAGE_BYTES;
+    uint64_t* afull = reinterpret_cast<uint64_t*>(codes + CODE_STAGES * CODE_BYTES);
     uint64_t* bfull = afull + STAGES;
     uint64_t* empty = bfull + STAGES;
     uint64_t* tfull = empty + STAGES;
     uint64_t* tempty = tfull + 2;
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tempty + 2);
+    uint64_t* cfull = tempty + 2;
+    uint64_t* cempty = cfull + CODE_STAGES;
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(cempty + CODE_STAGES);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
@@ -231,12 +169,16 @@ __global__ void __launch_bounds__(32 * (2 + (PIECES == 3 ? 8 : 4) + DQ_WARPS), 1
     if (threadIdx.x == 0) {
         for (int s = 0; s < STAGES; s++) {
             mbar_init(&afull[s], 1);
-            mbar_init(&bfull[s], 4 * CG);
+            mbar_init(&bfull[s], DQ_WARPS / 2 * CG);
             mbar_init(&empty[s], 1);
         }
         for (int b = 0; b < 2; b++) {
             mbar_init(&tfull[b], 1);
             mbar_init(&tempty[b], EW * CG);
+        }
+        for (int s = 0; s < CODE_STAGES; s++) {
+            mbar_init(&cfull[s], 1);
+            mbar_init(&cempty[s], DQ_WARPS);
         }
         *abort_flag = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -257,26 +199,23 @@ __global__ void __launch_bounds__(32 * (2 + (PIECES == 3 ? 8 : 4) + DQ_WARPS), 1
     const uint32_t tmem = *tmem_slot;
 
     const int units = a.tiles_m * a.tiles_n * a.splits;
-    uint32_t it = 0, cc = 0;  // stages and accumulators used so far, counted alike by every role
-    int pend[STAGES];
-#pragma unroll
-    for (int s = 0; s < STAGES; s++) pend[s] = -1;
+    uint32_t it = 0, ct = 0, cc = 0;  // stages, tiles of codes and accumulators used so far, counted alike by every role
     int commit_par[2] = {-1, -1};
 
-    // Calls body(kb, xp, wp, first, last) for each stage of a unit in ring order: first / last mark the stages that
-    // open and close an accumulator.  body returns false to stop.
-    auto stages = [&](const Unit& u, auto&& body) -> bool {
-        if constexpr (!FOLD) {
-            for (int kb = u.kb0; kb < u.kb1; kb++)
-                if (!body(kb, 0, 0, kb == u.kb0, kb == u.kb1 - 1)) return false;
+    // Calls body(kt, xp, wp, first, last) for each tile of a unit's contraction in ring order (one stage each): first /
+    // last mark the tiles that open and close an accumulator.  body returns false to stop.
+    auto tiles = [&](const Unit& u, auto&& body) -> bool {
+        if constexpr (!FOLDS) {
+            for (int kt = u.kt0; kt < u.kt1; kt++)
+                if (!body(kt, 0, 0, kt == u.kt0, kt == u.kt1 - 1)) return false;
         } else {
-            for (int c0 = u.kb0; c0 < u.kb1; c0 += FOLD_KB) {
-                const int c1 = min(u.kb1, c0 + FOLD_KB);
+            for (int c0 = u.kt0; c0 < u.kt1; c0 += FOLD) {
+                const int c1 = min(u.kt1, c0 + FOLD);
                 for (int c = 0; c < COMBOS; c++) {
                     int xp, wp;
                     combo(c, xp, wp);
-                    for (int kb = c0; kb < c1; kb++)
-                        if (!body(kb, xp, wp, c == 0 && kb == c0, c == COMBOS - 1 && kb == c1 - 1)) return false;
+                    for (int kt = c0; kt < c1; kt++)
+                        if (!body(kt, xp, wp, c == 0 && kt == c0, c == COMBOS - 1 && kt == c1 - 1)) return false;
                 }
             }
         }
@@ -289,20 +228,21 @@ __global__ void __launch_bounds__(32 * (2 + (PIECES == 3 ? 8 : 4) + DQ_WARPS), 1
             for (int un = worker; un < units && !*abort_flag; un += workers) {
                 const Unit u = unit_at<CG>(a, un);
                 const int row = (int)(u.m0 + rank * 128);
-                const bool ok = stages(u, [&](int kb, int xp, int, bool, bool) {
+                const bool ok = tiles(u, [&](int kt, int xp, int, bool, bool) {
                     const int s = it % STAGES;
-                    const uint32_t ph = (it / STAGES) & 1u;
-                    if (!mbar_wait(&empty[s], ph ^ 1u, abort_flag, a.err, a.wait_limit)) return false;
+                    if (!mbar_wait(&empty[s], ((it / STAGES) & 1u) ^ 1u, abort_flag, a.err, a.wait_limit)) return false;
                     unsigned char* dst = smem + s * STAGE_BYTES;
-                    const int y = row + (int)(xp * a.piece_rows);
+                    const int x = kt * TILE, y = row + (int)(xp * a.piece_rows);
                     if constexpr (CG == 2) {
                         if (rank == 0) mbar_expect_tx(&afull[s], 2 * A_BYTES);
-                        tma_load_2d_pair(dst, &amap, kb * BK, y, mapa_shared(smem_u32(&afull[s]), 0));
+                        const uint32_t bar = mapa_shared(smem_u32(&afull[s]), 0);
+                        tma_load_2d_pair(dst, &amap, x, y, bar);
+                        tma_load_2d_pair(dst + BOX_BYTES, &amap, x + BOX, y, bar);
                     } else {
                         mbar_expect_tx(&afull[s], A_BYTES);
-                        tma_load_2d(dst, &amap, kb * BK, y, &afull[s]);
+                        tma_load_2d(dst, &amap, x, y, &afull[s]);
+                        tma_load_2d(dst + BOX_BYTES, &amap, x + BOX, y, &afull[s]);
                     }
-                    pend[s] = (int)ph;
                     it++;
                     return true;
                 });
@@ -316,7 +256,7 @@ __global__ void __launch_bounds__(32 * (2 + (PIECES == 3 ? 8 : 4) + DQ_WARPS), 1
             for (int un = worker; un < units && !*abort_flag; un += workers) {
                 const Unit u = unit_at<CG>(a, un);
                 bool open = false;
-                const bool ok = stages(u, [&](int, int, int, bool first, bool last) {
+                const bool ok = tiles(u, [&](int, int, int, bool first, bool last) {
                     const int b = (int)(cc & 1u);
                     if (first) {
                         if (!mbar_wait(&tempty[b], ((cc >> 1) & 1u) ^ 1u, abort_flag, a.err, a.wait_limit)) return false;
@@ -326,28 +266,27 @@ __global__ void __launch_bounds__(32 * (2 + (PIECES == 3 ? 8 : 4) + DQ_WARPS), 1
                     const int s = it % STAGES;
                     const uint32_t ph = (it / STAGES) & 1u;
                     if (!mbar_wait(&afull[s], ph, abort_flag, a.err, a.wait_limit)) return false;
-                    if (CG == 2 ? !mbar_wait_cluster(&bfull[s], ph, abort_flag, a.err, a.wait_limit)
-                                : !mbar_wait(&bfull[s], ph, abort_flag, a.err, a.wait_limit))
-                        return false;
+                    if (!mbar_wait(&bfull[s], ph, abort_flag, a.err, a.wait_limit)) return false;
                     tc_fence_after();
                     const uint32_t abase = smem_u32(smem + s * STAGE_BYTES), bbase = abase + A_BYTES;
                     const uint32_t dst = tmem + (uint32_t)(b * BN);
 #pragma unroll
-                    for (int kk = 0; kk < BK / 16; kk++) {
-                        const uint64_t da = smem_desc_k_sw128(abase + kk * 32);
-                        const uint64_t db = DIR == 0 ? smem_desc_k_sw128(bbase + kk * 32) : smem_desc_mn_sw128(bbase + kk * 2048, 64 * BK * 2);
+                    for (int kk = 0; kk < TILE / 16; kk++) {
+                        const uint32_t k = kk / 4 * BOX_BYTES + kk % 4 * 32;  // K-major: 16 columns are 32 bytes of a box
+                        const uint64_t da = smem_desc_k_sw128(abase + k);
+                        const uint64_t db = DIR == 0 ? smem_desc_k_sw128(bbase + k) : smem_desc_mn_sw128(bbase + kk * 2048, BOX_BYTES);
                         const uint32_t acc = first && kk == 0 ? 0u : 1u;
                         if constexpr (CG == 2) umma2_f16(dst, da, db, a.idesc, acc);
                         else umma_f16(dst, da, db, a.idesc, acc);
                     }
                     commit<CG>(&empty[s]);
+                    it++;
                     if (last) {
                         commit<CG>(&tfull[b]);
                         commit_par[b] = (int)((cc >> 1) & 1u);
                         open = false;
                         cc++;
                     }
-                    it++;
                     return true;
                 });
                 if (!ok) {
@@ -363,7 +302,7 @@ __global__ void __launch_bounds__(32 * (2 + (PIECES == 3 ? 8 : 4) + DQ_WARPS), 1
     } else if (warp < 2 + EW) {
         // ---- epilogue: TMEM lane quadrant q, columns h EC ..
         const int q = warp % 4, h = (warp - 2) / 4;
-        float acc[FOLD ? EC : 1];
+        float acc[FOLDS ? EC : 1];
         for (int un = worker; un < units && !*abort_flag; un += workers) {
             const Unit u = unit_at<CG>(a, un);
             const int64_t tok = u.m0 + rank * 128 + q * 32 + lane;
@@ -377,9 +316,9 @@ __global__ void __launch_bounds__(32 * (2 + (PIECES == 3 ? 8 : 4) + DQ_WARPS), 1
                     if constexpr (Num<T>::MAGIC == Num<__half>::MAGIC) {
                         const int64_t col = col0 + i;
                         if (DIR == 0) {
-                            if (col < a.v.rows) o[i] *= pow2(a.v.exps[col]);
+                            if (col < a.v.rows) o[i] *= pow2(__ldg(a.v.exps + col));
                         } else {
-                            if (col < a.v.kp) o[i] *= pow2(a.v.exps[a.v.mp + group_of((int)col, a.v.gsv, a.v.groups)]);
+                            if (col < a.v.kp) o[i] *= pow2(__ldg(a.v.exps + a.v.mp + col / TILE * a.v.ng + slot_of((int)(col % TILE) / 32, a.v.ng)));
                         }
                     }
                 }
@@ -426,8 +365,8 @@ __global__ void __launch_bounds__(32 * (2 + (PIECES == 3 ? 8 : 4) + DQ_WARPS), 1
                     }
                 }
             };
-            const int chunks = FOLD ? (u.kb1 - u.kb0 + FOLD_KB - 1) / FOLD_KB : 1;
-            if constexpr (FOLD) {
+            const int chunks = FOLDS ? (u.kt1 - u.kt0 + FOLD - 1) / FOLD : 1;
+            if constexpr (FOLDS) {
 #pragma unroll
                 for (int i = 0; i < EC; i++) acc[i] = 0.f;
             }
@@ -445,7 +384,7 @@ __global__ void __launch_bounds__(32 * (2 + (PIECES == 3 ? 8 : 4) + DQ_WARPS), 1
                 for (int p = 0; p < EC / 32; p++) {
                     uint32_t r[32];
                     tmem_ld32(taddr + p * 32, r);
-                    if constexpr (FOLD) {
+                    if constexpr (FOLDS) {
 #pragma unroll
                         for (int i = 0; i < 32; i++) acc[p * 32 + i] = __fadd_rn(acc[p * 32 + i], __uint_as_float(r[i]));
                     } else {
@@ -463,7 +402,7 @@ __global__ void __launch_bounds__(32 * (2 + (PIECES == 3 ? 8 : 4) + DQ_WARPS), 1
                 }
             }
             if (!ok) break;
-            if constexpr (FOLD) {
+            if constexpr (FOLDS) {
 #pragma unroll
                 for (int p = 0; p < EC / 32; p++) {
                     float v[32];
@@ -473,50 +412,94 @@ __global__ void __launch_bounds__(32 * (2 + (PIECES == 3 ? 8 : 4) + DQ_WARPS), 1
                 }
             }
         }
-    } else {
-        // ---- dequantising: two groups of four warps take the 128-wide steps of the contraction in turn
-        const int grp = (warp - 2 - EW) / 4, tid = threadIdx.x - 32 * (2 + EW + 4 * grp);
+    } else if (warp < 2 + EW + DQ_WARPS) {
+        // ---- dequantising
+        const int grp = (warp - 2 - EW) / 4, w = (warp - 2 - EW) % 4, ng = a.v.ng, t = lane & 3, r8 = row_of(lane);
+        const int64_t lim = (DIR == 0 ? a.v.mp : a.v.kp) - 128;
         for (int un = worker; un < units && !*abort_flag; un += workers) {
             const Unit u = unit_at<CG>(a, un);
-            const int64_t n0 = u.n0 + rank * 128;
             // the last tile of a pair may reach past the padded weight: its columns are never stored
-            const int64_t lim = DIR == 0 ? a.v.mp : a.v.kp;
-            const int64_t nl = n0 < lim ? n0 : lim - 128;
-            int e[4] = {0, 0, 0, 0};
+            const int64_t nl = min(u.n0 + (int64_t)rank * 128, lim);
+            float e[4] = {1.f, 1.f, 1.f, 1.f};  // fp16: 2^-exponent of this thread's rows, or of the groups
             if constexpr (Num<T>::MAGIC == Num<__half>::MAGIC) {
-                if constexpr (DIR == 0) e[0] = a.v.exps[nl + tid];
-                else
 #pragma unroll
-                    for (int c = 0; c < 4; c++) e[c] = a.v.exps[a.v.mp + group_of((int)nl + 32 * c, a.v.gsv, a.v.groups)];
+                for (int c = 0; c < 4; c++)
+                    e[c] = pow2(-(DIR == 0 ? a.v.exps[nl + 32 * w + 8 * c + r8] : a.v.exps[a.v.mp + nl / TILE * ng + slot_of(c, ng)]));
             }
-            Frag f;
-            bool have = false;
-            const bool ok = stages(u, [&](int kb, int, int wp, bool, bool) {
-                const int s = it % STAGES;
+            const bool ok = tiles(u, [&](int, int, int wp, bool, bool) {
+                const int cs = ct % CODE_STAGES;
+                // The other group's tiles are waited for as well: copies may land out of order, and a stage of this ring
+                // changes hands every turn, so that a group that skipped one could take its old phase for the new one; and
+                // both let go of each, so that none is filled again before both have seen it full.
+                if (!mbar_wait(&cfull[cs], (ct / CODE_STAGES) & 1u, abort_flag, a.err, a.wait_limit)) return false;
+                ct++;
+                const int sg = it % STAGES;
                 const uint32_t ph = (it / STAGES) & 1u;
-                it++;
-                // A group follows the ring through the other's steps too: were it to skip their waits, units with few
-                // steps could leave it a whole turn of the ring behind, where the parity means the turn before.
-                if (((kb >> 1) & 1) != grp) return mbar_wait(&empty[s], ph ^ 1u, abort_flag, a.err, a.wait_limit);
-                if (!have) load_frag<DIR>(a.v, nl, kb, tid, f);
-                const Frag cur = f;
-                // the next step of this group within the unit, fetched while this one is converted
-                int nk = (kb & 1) ? kb + 3 : kb + 1;
-                have = false;
-                if constexpr (!FOLD) {
-                    if (nk < u.kb1) {
-                        load_frag<DIR>(a.v, nl, nk, tid, f);
-                        have = true;
+                if ((it++ & 1u) != (uint32_t)grp) {
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&cempty[cs]);
+                    return true;
+                }
+                const unsigned char* tile = codes + cs * CODE_BYTES;
+                uint4 q[4];
+                Scale<T, PIECES> sc[4][4];
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    const unsigned char* rec = tile + (2 * w + i / 2) * a.v.rec;
+                    const int in = 8 * (i & 1) + r8;
+                    q[i] = *reinterpret_cast<const uint4*>(rec + in * 64 + t * 16);
+                    const float* scales = reinterpret_cast<const float*>(rec + 1024) + in * ng;
+                    const unsigned char* zeros = rec + 1024 + 64 * ng + in * ng;
+#pragma unroll
+                    for (int c = 0; c < 4; c++) {
+                        if (c && ng == 1) {
+                            sc[i][c] = sc[i][0];
+                            continue;
+                        }
+                        sc[i][c].set(scales[slot_of(c, ng)] * e[DIR == 0 ? i : c], zeros[slot_of(c, ng)]);
                     }
                 }
-                if (!mbar_wait(&empty[s], ph ^ 1u, abort_flag, a.err, a.wait_limit)) return false;
-                store_frag<T, DIR, PIECES>(cur, smem + s * STAGE_BYTES + A_BYTES, tid, wp, e);
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&cempty[cs]);
+                if (!mbar_wait(&empty[sg], ph ^ 1u, abort_flag, a.err, a.wait_limit)) return false;
+                unsigned char* b = smem + sg * STAGE_BYTES + A_BYTES;
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    const uint32_t word[4] = {q[i].x, q[i].y, q[i].z, q[i].w};
+#pragma unroll
+                    for (int c = 0; c < 4; c++) {
+                        // K-major and MN-major alike: a box holds 64 layout columns of 128 rows, rows of 128 bytes
+                        const int off = c / 2 * BOX_BYTES + (32 * w + 8 * i + r8) * 128 + (((4 * (c & 1) + t) ^ r8) << 4);
+                        *reinterpret_cast<uint4*>(b + off) = dequant<T, PIECES>(word[c], sc[i][c], wp);
+                    }
+                }
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 __syncwarp();
+                // To the leader's barrier without a cluster-wide fence (with one the product took 1.6 times as long):
+                // what the arrival stands for is in this SM's own shared memory, complete for the async proxy by the
+                // fence above, and it is this SM's half of the MMA that reads it.
                 if (lane == 0) {
-                    if constexpr (CG == 2) mbar_arrive_cluster(mapa_shared(smem_u32(&bfull[s]), 0));
-                    else mbar_arrive(&bfull[s]);
+                    if constexpr (CG == 2) mbar_arrive_cluster_cta(mapa_shared(smem_u32(&bfull[sg]), 0));
+                    else mbar_arrive(&bfull[sg]);
                 }
+                return true;
+            });
+            if (!ok) break;
+        }
+    } else if (lane == 0) {
+        // ---- TMA: tiles of codes
+        const int64_t lim = (DIR == 0 ? a.v.mp : a.v.kp) - 128;
+        const uint32_t bytes = (uint32_t)(TILE / ROWS * a.v.rec);
+        for (int un = worker; un < units && !*abort_flag; un += workers) {
+            const Unit u = unit_at<CG>(a, un);
+            const int64_t nl = min(u.n0 + (int64_t)rank * 128, lim);
+            const bool ok = tiles(u, [&](int kt, int, int, bool, bool) {
+                const int cs = ct % CODE_STAGES;
+                if (!mbar_wait(&cempty[cs], ((ct / CODE_STAGES) & 1u) ^ 1u, abort_flag, a.err, a.wait_limit)) return false;
+                const int64_t at = DIR == 0 ? record_at(a.v, nl, kt) : record_at(a.v, (int64_t)kt * TILE, nl / TILE);
+                mbar_expect_tx(&cfull[cs], bytes);
+                bulk_load(codes + cs * CODE_BYTES, a.v.packed + at, bytes, &cfull[cs]);
+                ct++;
                 return true;
             });
             if (!ok) break;
@@ -526,11 +509,12 @@ __global__ void __launch_bounds__(32 * (2 + (PIECES == 3 ? 8 : 4) + DQ_WARPS), 1
     // Tail: no commit may still be on its way to a barrier of this CTA, nor, after an abort, a load to its memory.
     __syncwarp();
     if (warp == 0 && lane == 0)
-        for (int s = 0; s < STAGES; s++)
-            if (pend[s] >= 0) {
-                if (!*abort_flag) mbar_wait_drain(&empty[s], (uint32_t)pend[s]);
-                else if (rank == 0) mbar_wait_drain(&afull[s], (uint32_t)pend[s]);
-            }
+        for (uint32_t k = it > STAGES ? it - STAGES : 0; k < it; k++) {
+            if (!*abort_flag) mbar_wait_drain(&empty[k % STAGES], (k / STAGES) & 1u);
+            else if (rank == 0) mbar_wait_drain(&afull[k % STAGES], (k / STAGES) & 1u);
+        }
+    if (*abort_flag && warp == 2 + EW + DQ_WARPS && lane == 0)
+        for (uint32_t k = ct > CODE_STAGES ? ct - CODE_STAGES : 0; k < ct; k++) mbar_wait_drain(&cfull[k % CODE_STAGES], (k / CODE_STAGES) & 1u);
     if (*abort_flag && warp == 1 && lane == 0 && rank == 0)
         for (int b = 0; b < 2; b++)
             if (commit_par[b] >= 0) mbar_wait_drain(&tfull[b], (uint32_t)commit_par[b]);
@@ -601,7 +585,7 @@ template <auto kernel> int max_workers(llmc_ctx* ctx, int cg, int threads) {
 template <typename T, typename O, int DIR, int CG, int PIECES>
 llmc_status launch(llmc_ctx* ctx, cudaStream_t st, const CUtensorMap& map, GemmInt4& g) {
     constexpr auto kernel = gemm_int4_kernel<T, O, DIR, CG, PIECES>;
-    constexpr int threads = 32 * (2 + (PIECES == 3 ? 8 : 4) + DQ_WARPS);
+    constexpr int threads = 32 * (3 + (PIECES == 3 ? 8 : 4) + DQ_WARPS);
     int cap = max_workers<kernel>(ctx, CG, threads);
     const int allowed = persistent_sms(ctx) / CG;
     if (cap > allowed) cap = allowed;
@@ -628,17 +612,17 @@ llmc_status launch(llmc_ctx* ctx, cudaStream_t st, const CUtensorMap& map, GemmI
 // CTAs per tile for a product of this many tokens and columns.
 int int4_gemm_cg(int dtype, int64_t tokens, int64_t cols) { return dtype != LLMC_DTYPE_F32 && tokens > 128 && cols > 128 ? 2 : 1; }
 
-// Splits of the contraction: enough to give every worker a tile, four k-blocks to a split at least.
+// Splits of the contraction: enough to give every worker a tile, two tiles of 128 to a split at least.
 int int4_gemm_splits(const llmc_ctx* ctx, int dtype, int64_t tokens, int64_t cols, int64_t contraction) {
     const int cg = int4_gemm_cg(dtype, tokens, cols);
     const int64_t tile = 128 * cg, tiles = ((tokens + tile - 1) / tile) * ((cols + tile - 1) / tile);
-    const int64_t kb = (contraction + BK - 1) / BK, workers = persistent_sms(ctx) / cg;
+    const int64_t kt = contraction / TILE, workers = persistent_sms(ctx) / cg;
     int64_t s = workers / tiles;
-    if (s > kb / 4) s = kb / 4;
+    if (s > kt / 2) s = kt / 2;
     if (s > 32) s = 32;
     if (s < 1) s = 1;
-    const int64_t per = (kb + s - 1) / s;
-    return (int)((kb + per - 1) / per);
+    const int64_t per = (kt + s - 1) / s;
+    return (int)((kt + per - 1) / per);
 }
 
 // A [pieces][tokens][lda] 16-bit, K-major (see int4_stage for the pieces of fp32); out [tokens][ldo].
@@ -657,8 +641,8 @@ llmc_status int4_gemm(llmc_ctx* ctx, cudaStream_t st, const w4::View& v, int dir
     g.tiles_m = (int)((tokens + tile - 1) / tile);
     g.tiles_n = (int)((cols + tile - 1) / tile);
     g.splits = splits;
-    g.kb_total = (int)(contraction / BK);
-    g.kb_per = (g.kb_total + splits - 1) / splits;
+    g.kt_total = (int)(contraction / TILE);
+    g.kt_per = (g.kt_total + splits - 1) / splits;
     g.group_m = 8;
     g.piece_rows = tokens;
     g.bias = splits > 1 ? nullptr : bias;
@@ -675,7 +659,7 @@ llmc_status int4_gemm(llmc_ctx* ctx, cudaStream_t st, const w4::View& v, int dir
     CUtensorMap map;
     const cuuint64_t dim[2] = {(cuuint64_t)acols, (cuuint64_t)(tokens * pieces)};
     const cuuint64_t stride[1] = {(cuuint64_t)lda * 2};
-    const cuuint32_t box[2] = {BK, 128}, es1[2] = {1, 1};
+    const cuuint32_t box[2] = {BOX, 128}, es1[2] = {1, 1};
     const CUresult cr = enc(&map, fmt ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, const_cast<void*>(A), dim, stride,
                             box, es1, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);

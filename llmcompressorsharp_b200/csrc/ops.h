@@ -70,8 +70,8 @@ llmc_status ct_pack(llmc_ctx* ctx, const uint8_t* codes, int64_t m, int64_t n, i
 // These and the embedding's take their stream from the caller and use none of the context's
 // workspaces, so calls on several streams and captured ones do not share memory.
 llmc_status int4_layout(llmc_ctx* ctx, cudaStream_t st, const uint8_t* codes, int64_t crow, const float* scales,
-                        const int32_t* zps, int64_t srow, int sym, const w4::View& v, uint32_t* packed, float* sout,
-                        uint8_t* zout, int32_t* exps);
+                        const int32_t* zps, int64_t srow, int sym, const w4::View& v, uint8_t* packed,
+                        int32_t* exps);
 // out[t] = scale * W[ids[t]] (ids null: row t).
 llmc_status int4_rows(llmc_ctx* ctx, cudaStream_t st, const w4::View& v, const void* ids, int ids64, int64_t tokens,
                       float scale, void* out, int dtype, int64_t ldo);

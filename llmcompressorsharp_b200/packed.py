@@ -74,8 +74,8 @@ class Int4Weight:
             raise InvalidOperationError("a packed weight's scales take no gradient")
         rows = codes.shape[0]
         group = int(group_size) if strategy == "group" else max(1, int(cols))
-        words, entries, exps = _lib.I64(), _lib.I64(), _lib.I64()
-        _lib.call("llmc_int4_layout_sizes", rows, cols, group, C.byref(words), C.byref(entries), C.byref(exps))
+        size, exps = _lib.I64(), _lib.I64()
+        _lib.call("llmc_int4_layout_sizes", rows, cols, group, C.byref(size), C.byref(exps))
         want = {"tensor": 1, "channel": rows, "group": rows * -(-cols // group)}[strategy]
         for name, t in (("scales", scales), ("zero_points", zero_points)):
             if t is not None and t.numel() != want:
@@ -88,12 +88,9 @@ class Int4Weight:
         c = to_device(codes.detach(), self.device)
         s = to_device(scales.detach(), self.device, torch.float32)
         z = to_device(zero_points.detach(), self.device, torch.int32) if not symmetric else None
-        self.packed = torch.empty(words.value, dtype=torch.int32, device=self.device)
-        self.scales = torch.empty(entries.value, dtype=torch.float32, device=self.device)
-        self.zeros = torch.empty(entries.value, dtype=torch.uint8, device=self.device)
+        self.packed = torch.empty(size.value, dtype=torch.uint8, device=self.device)
         self.exps = torch.empty(exps.value, dtype=torch.int32, device=self.device)
-        self._c = _lib.Int4WeightC(self.packed.data_ptr(), self.scales.data_ptr(), self.zeros.data_ptr(),
-                                   self.exps.data_ptr(), rows, int(cols), group)
+        self._c = _lib.Int4WeightC(self.packed.data_ptr(), self.exps.data_ptr(), rows, int(cols), group)
         self._ref = C.byref(self._c)
         self._ctx, self._index = _lib.ctx_handle(self.device.index), self.device.index
         self._need: dict = {}

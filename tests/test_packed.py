@@ -71,19 +71,21 @@ def test_layout_sizes_and_their_refusals():
     from llmcompressorsharp_b200 import _lib
 
     lib = _lib.load()
-    w, e, x = C.c_int64(), C.c_int64(), C.c_int64()
+    p, x = C.c_int64(), C.c_int64()
 
     def sizes(rows, cols, group):
-        return lib.llmc_int4_layout_sizes(rows, cols, group, C.byref(w), C.byref(e), C.byref(x))
+        return lib.llmc_int4_layout_sizes(rows, cols, group, C.byref(p), C.byref(x))
 
-    assert sizes(100, 576, 128) == 0 and (w.value, e.value, x.value) == (128 * 640 // 8, 128 * 5, 128 + 5)
-    # 12 groups of 50 columns take 64 each, the last one 50 - rounded up to 128 columns in all
-    assert sizes(129, 600, 50) == 0 and (w.value, e.value, x.value) == (256 * 768 // 8, 256 * 12, 256 + 12)
-    assert sizes(1, 5, 8) == 0 and (w.value, e.value) == (128 * 128 // 8, 128)
+    # records of 16 rows x 128 columns: 1,024 bytes of codes, 80 for each group in the 128 columns
+    assert sizes(100, 576, 128) == 0 and (p.value, x.value) == (8 * 5 * 1104, 128 + 5)
+    # twelve groups of 50 columns take 64 each: two to a record
+    assert sizes(129, 600, 50) == 0 and (p.value, x.value) == (16 * 6 * 1184, 256 + 12)
+    assert sizes(16, 96, 32) == 0 and (p.value, x.value) == (8 * 1344, 128 + 4)
+    assert sizes(1, 5, 8) == 0 and (p.value, x.value) == (8 * 1104, 128 + 1)
     assert sizes(0, 5, 8) == 2 and sizes(5, 0, 8) == 2  # LLMC_ERR_SHAPE
     assert sizes(5, 64, 15) == 3  # LLMC_ERR_UNSUPPORTED
     assert sizes(1 << 31, 64, 64) == 10  # LLMC_ERR_OUT_OF_RANGE
-    assert lib.llmc_int4_layout_sizes(4, 4, 4, None, None, None) == 1
+    assert lib.llmc_int4_layout_sizes(4, 4, 4, None, None) == 1
 
 
 def test_null_arguments_are_statuses():
@@ -424,6 +426,6 @@ def test_call_refusals():
         _lib.call("llmc_int4_linear", *args, None, 0)
     with pytest.raises(ShapeError):
         _lib.call("llmc_int4_linear", *args[:6], 63, *args[7:], None, 0)
-    bad = _lib.Int4WeightC(p.packed.data_ptr(), p.scales.data_ptr(), p.zeros.data_ptr(), p.exps.data_ptr(), 20, 64, 8)
+    bad = _lib.Int4WeightC(p.packed.data_ptr(), p.exps.data_ptr(), 20, 64, 8)
     with pytest.raises(NotSupportedError):
         _lib.call("llmc_int4_linear", *args[:2], C.byref(bad), *args[3:], None, 0)
