@@ -18,8 +18,9 @@
 //           size; a group of 256 columns or more has its scale in each tile)
 //   zeros   16 rows x ng bytes
 //
-// So whatever a product needs for 16 rows x 128 columns is one stretch of 1,104 bytes (ng = 1), which one bulk
-// copy brings in, and nothing is fetched from a second place with a latency of its own.
+// So whatever a product needs of a tile is one stretch of 8,832 bytes (ng = 1), which one bulk copy brings in, and
+// nothing comes from a second place with a latency of its own.  (Records that stood along the columns instead, for
+// eight copies to a tile, made the products of many rows a fifth slower: a bulk copy costs its issue.)
 #pragma once
 #include "common.cuh"
 
@@ -70,7 +71,7 @@ __host__ __device__ __forceinline__ int group_of(int kv, int gsv, int groups) {
     return g < groups ? g : groups - 1;
 }
 
-// Record of row r's 16 rows in the tile of columns 128 kt ..
+// Byte at which the record of row r's 16 rows and columns 128 kt .. stands.
 __host__ __device__ __forceinline__ int64_t record_at(const View& v, int64_t r, int64_t kt) {
     return ((r / TILE * (v.kp / TILE) + kt) * (TILE / ROWS) + r % TILE / ROWS) * v.rec;
 }
@@ -113,11 +114,25 @@ template <typename T> __device__ __forceinline__ uint32_t zero_pair(uint32_t z) 
     return Num<T>::MAGIC | z | (z << 16);
 }
 
+// The operands of int_pair's logic operation, in registers: as literals the compiler, which can put one into an
+// instruction, fetches the other anew for each pair, a fourth instruction on the three that a pair takes.  They come
+// through shared memory (`slot`, written by one thread before a barrier) to hide their values from it.
+struct Bits {
+    uint32_t mask, magic;
+};
+template <typename T> __device__ __forceinline__ void put_bits(uint2* slot) { *slot = make_uint2(0x000F000Fu, Num<T>::MAGIC); }
+__device__ __forceinline__ Bits get_bits(const uint2* slot) {
+    Bits b;
+    asm volatile("ld.volatile.shared.v2.u32 {%0, %1}, [%2];"
+                 : "=r"(b.mask), "=r"(b.magic)
+                 : "r"(static_cast<uint32_t>(__cvta_generic_to_shared(slot))));
+    return b;
+}
+
 // Pair p (columns 2 p, 2 p + 1) of a word as the two integers u - z in T.
-template <typename T> __device__ __forceinline__ uint32_t int_pair(uint32_t word, int p, uint32_t zz) {
+template <typename T> __device__ __forceinline__ uint32_t int_pair(uint32_t word, int p, uint32_t zz, Bits k) {
     uint32_t m;
-    // (word >> 4p) & mask | magic is one shift and one three-input logic operation
-    asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(m) : "r"(word >> (4 * p)), "r"(0x000F000Fu), "r"(Num<T>::MAGIC));
+    asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(m) : "r"(word >> (4 * p)), "r"(k.mask), "r"(k.magic));
     return bits2(__hsub2(as2<T>(m), as2<T>(zz)));
 }
 

@@ -7,8 +7,6 @@
 #include "ops.h"
 #include "tc_common.cuh"
 
-#include <atomic>
-
 namespace llmc {
 namespace {
 
@@ -207,15 +205,17 @@ __global__ void __launch_bounds__(256) stage_kernel(const T* x, int64_t tokens, 
 }
 
 // ---- products with few rows ---------------------------------------------------------------------
-__device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, __nv_bfloat16) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-__device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, __half) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+// d = a b + c, with c = 0 where `fresh`.
+template <typename T> __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, bool fresh) {
+    const float c0 = fresh ? 0.f : d[0], c1 = fresh ? 0.f : d[1], c2 = fresh ? 0.f : d[2], c3 = fresh ? 0.f : d[3];
+    if constexpr (Num<T>::MAGIC == Num<__half>::MAGIC)
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};"
+                     : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+                     : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(c0), "f"(c1), "f"(c2), "f"(c3));
+    else
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};"
+                     : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+                     : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(c0), "f"(c1), "f"(c2), "f"(c3));
 }
 
 struct FewArgs {
@@ -226,191 +226,158 @@ struct FewArgs {
     const void* bias;
     void* y;
     int64_t ldy;
-    int* err;
-    uint32_t wait_limit;
 };
 
-constexpr int RING = 4;       // steps in flight per warp
-constexpr int few_warps(int rb) { return 16 / rb; }  // per CTA at most
+constexpr int FEW_WARPS = 8;  // per CTA at most
+__host__ __device__ constexpr int few_stages(int rb) { return rb == 1 ? 5 : 3; }
+
+__device__ __forceinline__ void copy16(void* dst, const void* src, int bytes) {  // bytes < 16: zeros for the rest
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(tc::smem_u32(dst)), "l"(src), "r"(bytes) : "memory");
+}
 
 // The codes are the A operand of m16n8k16 (16 weight rows x 16 columns), x the B operand (8 tokens), so one
 // dequantised fragment serves eight tokens and a single token costs no more than the codes.  Codes enter as
 // the exact integers u - z; the fp32 sum of a group is multiplied by its scale (4 / NG granules of 32 columns per
-// group sum), so x and W are never rounded.
-// A CTA holds RB records' rows (16 RB) and 8 NT tokens at a time; its warps take the 128-column steps in turn, each
-// through a ring of its own that bulk copies keep full across rows, and add their sums in shared memory, in warp order.
+// group sum), so x and W are never rounded.  Columns of the MMA that stand for no token repeat the last one's x.
+// A CTA holds RB records' rows (16 RB) and 8 NT tokens; its warps take the 128-column steps in turn and add their sums
+// in shared memory, in warp order.  Each warp keeps a ring of STAGES steps in flight, the records and the 256 bytes
+// of each token's x (XS), by 16-byte asynchronous copies that it waits for by itself.  The three pieces of fp32 x would
+// take most of the ring and are read through L1, which row blocks of few columns share.
+// What bounds it is the instructions: at the HBM's rate an SM has 43 clocks for a record, 172 issue slots, of which
+// turning its codes into numbers takes 88.
 template <typename T, typename O, int NT, int PIECES, int NG, int RB>
-__global__ void __launch_bounds__(32 * few_warps(RB)) few_kernel(const FewArgs a) {
-    constexpr int REC = 1024 + 80 * NG, STEP = RB * REC, FL = 4 / NG, SUMS = 8 * NT * ROWS * RB;
-    extern __shared__ __align__(128) uint8_t smem[];  // rings, barriers, two [warps][8 NT][16 RB] of sums
+__global__ void __launch_bounds__(32 * FEW_WARPS) few_kernel(const FewArgs a) {
+    constexpr int REC = 1024 + 80 * NG, FL = 4 / NG, SUMS = 8 * NT * ROWS * RB, STAGES = few_stages(RB);
+    constexpr bool XS = PIECES == 1;
+    extern __shared__ __align__(128) uint8_t smem[];  // int_pair's operands, rings; afterwards [warps][8 NT][16 RB] of sums
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, warps = blockDim.x / 32;
-    uint8_t* ring = smem + warp * RING * STEP;
-    uint64_t* bars = reinterpret_cast<uint64_t*>(smem + warps * RING * STEP) + warp * RING;
-    float* red = reinterpret_cast<float*>(smem + warps * RING * (STEP + 8));
     const int g = lane >> 2, t = lane & 3;
+    const int tok0 = blockIdx.y * 8 * NT, toks = min(8 * NT, a.tokens - tok0);
+    const int64_t row0 = (int64_t)blockIdx.x * (ROWS * RB);
     const int ktiles = (int)(a.v.kp / TILE);
-    const int blocks = (int)((a.v.rows + ROWS * RB - 1) / (ROWS * RB));
-    const int tok0 = blockIdx.y * 8 * NT;
-    if (lane == 0) {
-        for (int s = 0; s < RING; s++) tc::mbar_init(&bars[s], 1);
-        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-    }
-    __syncwarp();
+    const int room = RB * REC + (XS ? toks * 256 : 0);
+    uint8_t* ring = smem + 16 + warp * STAGES * room;
+    if (threadIdx.x == 0) put_bits<T>(reinterpret_cast<uint2*>(smem));
+    __syncthreads();
+    const Bits bits = get_bits(reinterpret_cast<const uint2*>(smem));
 
-    // the next step to fetch: row block prb, tile pkt, in the ring's stage pst
-    int prb = blockIdx.x, pkt = warp, pst = 0;
-    uint32_t fetched = 0, used = 0;
-    bool failed = false;
-    const uint8_t* src = a.v.packed + record_at(a.v, (int64_t)prb * (ROWS * RB), pkt);
-    const int64_t hop = (int64_t)warps * (TILE / ROWS) * REC;
-    auto fetch = [&]() {
-        if (prb >= blocks || failed) return;
-        if (lane == 0) {
-            tc::mbar_expect_tx(&bars[pst], STEP);
-            tc::bulk_load(ring + pst * STEP, src, STEP, &bars[pst]);
+    int fkt = warp;  // the step to fetch next
+    const uint8_t* src = a.v.packed + record_at(a.v, row0, warp) + lane * 16;
+    const T* xsrc = reinterpret_cast<const T*>(a.x) + (int64_t)(tok0 + lane / 16) * a.ldx + warp * TILE + lane % 16 * 8;
+    auto fetch = [&](uint8_t* stage) {
+        if (fkt < ktiles) {
+            uint8_t* dst = stage + lane * 16;
+#pragma unroll
+            for (int i = 0; i < RB * REC / 512; i++) copy16(dst + i * 512, src + i * 512, 16);
+            if (lane < RB * REC % 512 / 16) copy16(dst + RB * REC / 512 * 512, src + RB * REC / 512 * 512, 16);
+            if (XS) {
+                // two tokens' 256 bytes to a copy; zeros past the last column
+                const bool in = fkt * TILE + lane % 16 * 8 < a.xcols;
+                const T* xr = in ? xsrc : reinterpret_cast<const T*>(a.x);
+                const int64_t two = in ? 2 * a.ldx : 0;
+                for (int r = lane / 16; r < toks; r += 2, xr += two) copy16(stage + RB * REC + r * 256 + lane % 16 * 16, xr, in ? 16 : 0);
+            }
+            fkt += warps;
+            src += (int64_t)warps * (TILE / ROWS) * REC;
+            xsrc += warps * TILE;
         }
-        fetched++;
-        pst = pst == RING - 1 ? 0 : pst + 1;
-        pkt += warps;
-        src += hop;
-        if (pkt >= ktiles) {
-            pkt = warp;
-            prb += gridDim.x;
-            src = a.v.packed + record_at(a.v, (int64_t)prb * (ROWS * RB), pkt);
-        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
     };
-    for (int s = 0; s < RING; s++) fetch();
+#pragma unroll
+    for (int s = 0; s < STAGES - 1; s++) fetch(ring + s * room);
 
-    // this lane's token of each eight and piece, at its columns of the first granule
-    const T* xp[NT][PIECES];
+    int xat[NT];  // this lane's token of each eight in a stage, or (in elements) in x
 #pragma unroll
-    for (int n = 0; n < NT; n++)
-#pragma unroll
-        for (int p = 0; p < PIECES; p++) {
-            const int tok = tok0 + n * 8 + g;
-            xp[n][p] = tok < a.tokens ? reinterpret_cast<const T*>(a.x) + ((int64_t)p * a.tokens + tok) * a.ldx + 8 * t : nullptr;
-        }
-    auto load_x = [&](int kt, uint4 (&b)[4][NT][PIECES]) {
-#pragma unroll
-        for (int c = 0; c < 4; c++)
-#pragma unroll
-            for (int n = 0; n < NT; n++)
-#pragma unroll
-                for (int p = 0; p < PIECES; p++) {
-                    const int k = kt * TILE + 32 * c;
-                    b[c][n][p] = make_uint4(0, 0, 0, 0);
-                    if (xp[n][p] && k + 8 * t < a.xcols) b[c][n][p] = __ldg(reinterpret_cast<const uint4*>(xp[n][p] + k));
-                }
+    for (int n = 0; n < NT; n++) xat[n] = min(n * 8 + g, toks - 1);
+    auto load_x = [&](const uint8_t* stage, int kt, int c, int n, int p) {
+        if (XS) return *reinterpret_cast<const uint4*>(stage + RB * REC + xat[n] * 256 + t * 16 + c * 64);
+        const int k = kt * TILE + 32 * c + 8 * t;
+        if (k >= a.xcols) return make_uint4(0, 0, 0, 0);
+        return __ldg(reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(a.x) + ((int64_t)p * a.tokens + tok0 + xat[n]) * a.ldx + k));
     };
-    constexpr bool AHEAD = NT * PIECES <= 2;  // 16 registers for each of NT and PIECES
-    uint4 nb[4][NT][PIECES];
-    if constexpr (AHEAD) load_x(warp, nb);
-    int flip = 0, st = 0;
-    for (int rb = blockIdx.x; rb < blocks; rb += gridDim.x, flip ^= 1) {
-        float acc[RB][NT][4];
+    float acc[RB][NT][4];
+#pragma unroll
+    for (int r = 0; r < RB; r++)
+#pragma unroll
+        for (int n = 0; n < NT; n++)
+#pragma unroll
+            for (int j = 0; j < 4; j++) acc[r][n][j] = 0.f;
+    int at = 0, to = (STAGES - 1) * room;  // the stages to multiply and to fill
+    for (int kt = warp; kt < ktiles; kt += warps) {
+        asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 2) : "memory");
+        __syncwarp();
+        fetch(ring + to);
+        const uint8_t* stage = ring + at;
+        at = at == (STAGES - 1) * room ? 0 : at + room;
+        to = to == (STAGES - 1) * room ? 0 : to + room;
+        uint32_t w[RB][2][4], zz[RB][2][NG];
+        float sc[RB][2][NG];
 #pragma unroll
         for (int r = 0; r < RB; r++)
 #pragma unroll
+            for (int h = 0; h < 2; h++) {
+                const uint8_t* q = stage + r * REC;
+                const int row = g + 8 * h;
+                const uint4 u = *reinterpret_cast<const uint4*>(q + row * 64 + t * 16);
+                w[r][h][0] = u.x;
+                w[r][h][1] = u.y;
+                w[r][h][2] = u.z;
+                w[r][h][3] = u.w;
+#pragma unroll
+                for (int j = 0; j < NG; j++) {
+                    sc[r][h][j] = reinterpret_cast<const float*>(q + 1024)[row * NG + j];
+                    zz[r][h][j] = q[1024 + 64 * NG + row * NG + j] * 0x10001u + bits.magic;
+                }
+            }
+        float d[RB][NT][4];
+#pragma unroll
+        for (int c = 0; c < 4; c++) {
+            const int j = c / FL;
+            uint4 b[NT][PIECES];
+#pragma unroll
             for (int n = 0; n < NT; n++)
 #pragma unroll
-                for (int j = 0; j < 4; j++) acc[r][n][j] = 0.f;
-        for (int kt = warp; kt < ktiles && !failed; kt += warps) {
-            uint4 b[4][NT][PIECES];
-            if constexpr (AHEAD) {
-                // the next step's x while this one is multiplied: with one row block to a CTA each of these is a miss of L1
+                for (int p = 0; p < PIECES; p++) b[n][p] = load_x(stage, kt, c, n, p);
 #pragma unroll
-                for (int c = 0; c < 4; c++)
+            for (int r = 0; r < RB; r++) {
+                uint32_t f[2][4];
 #pragma unroll
-                    for (int n = 0; n < NT; n++)
+                for (int h = 0; h < 2; h++)
 #pragma unroll
-                        for (int p = 0; p < PIECES; p++) b[c][n][p] = nb[c][n][p];
-                load_x(kt + warps < ktiles ? kt + warps : warp, nb);
-            } else {
-                load_x(kt, b);
-            }
-            if (!tc::mbar_wait_bounded(&bars[st], (used / RING) & 1u, a.wait_limit)) failed = true;
-            if (__any_sync(0xffffffffu, failed)) {
-                failed = true;
-                break;
-            }
-            used++;
-            const uint8_t* rec = ring + st * STEP;
-            st = st == RING - 1 ? 0 : st + 1;
-            uint32_t w[RB][2][4], zz[RB][2][NG];
-            float sc[RB][2][NG];
+                    for (int k = 0; k < 4; k++) f[h][k] = int_pair<T>(w[r][k & 1][c], 2 * h + k / 2, zz[r][k & 1][j], bits);
 #pragma unroll
-            for (int r = 0; r < RB; r++)
+                for (int n = 0; n < NT; n++)
 #pragma unroll
-                for (int i = 0; i < 2; i++) {
-                    const int row = g + 8 * i;
-                    const uint8_t* q = rec + r * REC;
-                    const uint4 u = *reinterpret_cast<const uint4*>(q + row * 64 + t * 16);
-                    w[r][i][0] = u.x;
-                    w[r][i][1] = u.y;
-                    w[r][i][2] = u.z;
-                    w[r][i][3] = u.w;
-#pragma unroll
-                    for (int j = 0; j < NG; j++) {
-                        sc[r][i][j] = reinterpret_cast<const float*>(q + 1024)[row * NG + j];
-                        zz[r][i][j] = zero_pair<T>(q[1024 + 64 * NG + row * NG + j]);
+                    for (int p = PIECES - 1; p >= 0; p--) {
+                        mma16816<T>(d[r][n], f[0], b[n][p].x, b[n][p].y, c % FL == 0 && p == PIECES - 1);
+                        mma16816<T>(d[r][n], f[1], b[n][p].z, b[n][p].w, false);
                     }
-                }
-            __syncwarp();
-            fetch();  // into the stage just read
-            float d[RB][NT][4];
-#pragma unroll
-            for (int c = 0; c < 4; c++) {
-                const int j = c / FL;
-#pragma unroll
-                for (int r = 0; r < RB; r++) {
-                    if (c % FL == 0)
-#pragma unroll
-                        for (int n = 0; n < NT; n++)
-#pragma unroll
-                            for (int i = 0; i < 4; i++) d[r][n][i] = 0.f;
-                    uint32_t f[2][4];
-#pragma unroll
-                    for (int h = 0; h < 2; h++)
-#pragma unroll
-                        for (int i = 0; i < 4; i++) f[h][i] = int_pair<T>(w[r][i & 1][c], 2 * h + i / 2, zz[r][i & 1][j]);
+                if (c % FL == FL - 1)
 #pragma unroll
                     for (int n = 0; n < NT; n++)
 #pragma unroll
-                        for (int p = PIECES - 1; p >= 0; p--) {
-                            mma16816(d[r][n], f[0], b[c][n][p].x, b[c][n][p].y, T());
-                            mma16816(d[r][n], f[1], b[c][n][p].z, b[c][n][p].w, T());
-                        }
-                    if (c % FL == FL - 1)
-#pragma unroll
-                        for (int n = 0; n < NT; n++)
-#pragma unroll
-                            for (int i = 0; i < 4; i++) acc[r][n][i] = fmaf(sc[r][i / 2][j], d[r][n][i], acc[r][n][i]);
-                }
+                        for (int k = 0; k < 4; k++) acc[r][n][k] = fmaf(sc[r][k / 2][j], d[r][n][k], acc[r][n][k]);
             }
         }
-        float* sums = red + flip * warps * SUMS;
-#pragma unroll
-        for (int r = 0; r < RB; r++)
-#pragma unroll
-            for (int n = 0; n < NT; n++)
-#pragma unroll
-                for (int i = 0; i < 4; i++)  // [warp][token][row]
-                    sums[warp * SUMS + (n * 8 + 2 * t + (i & 1)) * (ROWS * RB) + r * ROWS + g + 8 * (i / 2)] = acc[r][n][i];
-        __syncthreads();  // the other buffer's readers have all passed the sync before this one
-        for (int i = threadIdx.x; i < SUMS; i += blockDim.x) {
-            const int64_t row = (int64_t)rb * (ROWS * RB) + i % (ROWS * RB);
-            const int tok = tok0 + i / (ROWS * RB);
-            if (row >= a.v.rows || tok >= a.tokens) continue;
-            float s = 0.f;
-            for (int w = 0; w < warps; w++) s += sums[w * SUMS + i];
-            if (a.bias) s += to_f<O>(reinterpret_cast<const O*>(a.bias)[row]);
-            reinterpret_cast<O*>(a.y)[tok * a.ldy + row] = from_f<O>(s);
-        }
     }
-    // after a wait that gave up, copies may still be on their way
-    if (failed) {
-        atomicOr(a.err, 1);
-        for (; used < fetched; used++) tc::mbar_wait_drain(&bars[used % RING], (used / RING) & 1u);
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
+    __syncthreads();  // the rings are done with
+    float* red = reinterpret_cast<float*>(smem);
+#pragma unroll
+    for (int r = 0; r < RB; r++)
+#pragma unroll
+        for (int n = 0; n < NT; n++)
+#pragma unroll
+            for (int i = 0; i < 4; i++)  // [warp][token][row]
+                red[warp * SUMS + (n * 8 + 2 * t + (i & 1)) * (ROWS * RB) + r * ROWS + g + 8 * (i / 2)] = acc[r][n][i];
+    __syncthreads();
+    for (int i = threadIdx.x; i < toks * (ROWS * RB); i += blockDim.x) {
+        const int64_t row = row0 + i % (ROWS * RB);
+        if (row >= a.v.rows) continue;
+        float s = 0.f;
+        for (int w = 0; w < warps; w++) s += red[w * SUMS + i];
+        if (a.bias) s += to_f<O>(reinterpret_cast<const O*>(a.bias)[row]);
+        reinterpret_cast<O*>(a.y)[(tok0 + i / (ROWS * RB)) * a.ldy + row] = from_f<O>(s);
     }
 }
 
@@ -453,54 +420,38 @@ int grid_n(const llmc_ctx* ctx, int64_t items) {
     return (int)(b < 1 ? 1 : (b > cap ? cap : b));
 }
 
-// CTAs of `threads` that an SM holds; asked once per kernel and number of warps.
-template <auto kernel> int resident(int device, int warps, size_t smem) {
-    static std::atomic<int> known[64][few_warps(1) + 1];
-    if (device < 0 || device >= 64) return 1;
-    int n = known[device][warps].load(std::memory_order_relaxed);
-    if (n == 0) {
-        if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024) != cudaSuccess ||
-            cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kernel, warps * 32, smem) != cudaSuccess || n < 1) {
-            cudaGetLastError();
-            return 0;
-        }
-        known[device][warps].store(n, std::memory_order_relaxed);
-    }
-    return n;
-}
-
 template <typename T, typename O, int NT, int PIECES, int NG, int RB>
 llmc_status launch_few(llmc_ctx* ctx, const FewArgs& a, cudaStream_t st) {
-    constexpr int STEP = RB * (1024 + 80 * NG);
+    constexpr auto kernel = few_kernel<T, O, NT, PIECES, NG, RB>;
+    constexpr int REC = 1024 + 80 * NG, STAGES = few_stages(RB);
     const int64_t blocks = (a.v.rows + ROWS * RB - 1) / (ROWS * RB);
     const int ktiles = (int)(a.v.kp / TILE), tiles = (a.tokens + 8 * NT - 1) / (8 * NT);
-    // sixteen warps to a CTA where the rows give an SM two CTAs or fewer, eight where they give more: see few_kernel
-    const int most = blocks * tiles <= 2 * ctx->sm_count ? few_warps(RB) : 8;
-    const int warps = ktiles < most ? ktiles : most;
-    constexpr int SUMS = 2 * 8 * NT * ROWS * RB * (int)sizeof(float);
-    static_assert(few_warps(RB) * (RING * (STEP + 8) + SUMS) <= 227 * 1024, "shared memory of an SM");
-    const size_t sm = (size_t)warps * (RING * (STEP + 8) + SUMS);
-    constexpr auto kernel = few_kernel<T, O, NT, PIECES, NG, RB>;
-    const int per = resident<kernel>(ctx->device, warps, sm);
-    if (per < 1) return fail(LLMC_ERR_CUDA, "the packed product's kernel does not fit this device");
-    int64_t cap = (int64_t)per * persistent_sms(ctx) / tiles;
-    if (cap < 1) cap = 1;
-    kernel<<<dim3((unsigned)(blocks < cap ? blocks : cap), (unsigned)tiles), warps * 32, sm, st>>>(a);
+    const int warps = ktiles < FEW_WARPS ? ktiles : FEW_WARPS, toks = a.tokens < 8 * NT ? a.tokens : 8 * NT;
+    size_t sm = 16 + (size_t)warps * STAGES * (RB * REC + (PIECES == 1 ? toks * 256 : 0)), sums = (size_t)warps * 8 * NT * ROWS * RB * sizeof(float);
+    if (sm < sums) sm = sums;
+    static_assert(16 + FEW_WARPS * STAGES * (RB * REC + (PIECES == 1 ? 8 * NT * 256 : 0)) <= 227 * 1024, "shared memory of an SM");
+    LLMC_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sm));
+    kernel<<<dim3((unsigned)blocks, (unsigned)tiles), warps * 32, sm, st>>>(a);
     return check_launch(ctx, "int4_few");
 }
 
-template <typename T, typename O, int NT, int PIECES, int RB>
-llmc_status few_by_group(llmc_ctx* ctx, const FewArgs& a, cudaStream_t st) {
+template <typename T, typename O, int NT, int PIECES, int RB> llmc_status few_by_group(llmc_ctx* ctx, const FewArgs& a, cudaStream_t st) {
     if (a.v.ng == 1) return launch_few<T, O, NT, PIECES, 1, RB>(ctx, a, st);
     if (a.v.ng == 2) return launch_few<T, O, NT, PIECES, 2, RB>(ctx, a, st);
     return launch_few<T, O, NT, PIECES, 4, RB>(ctx, a, st);
 }
 
 template <typename T, typename O, int PIECES> llmc_status few_by_size(llmc_ctx* ctx, const FewArgs& a, cudaStream_t st) {
-    // Two records a step share the loads of x (NT PIECES x 2 KB a step from L1, against 1 KB of codes a record); with few
-    // rows one, which makes twice the CTAs.
-    if (a.tokens > 8) return few_by_group<T, O, 2, PIECES, 2>(ctx, a, st);
-    return few_by_group<T, O, 1, PIECES, 1>(ctx, a, st);
+    if constexpr (PIECES == 1) {
+        if (a.tokens > 8) {
+            // x is 256 bytes a token beside a record's 1,104: with many tokens several records share it, as long as the
+            // rows still give every SM a CTA
+            const int64_t blocks = (a.v.rows + ROWS - 1) / ROWS * ((a.tokens + 15) / 16);
+            if (blocks >= 4 * ctx->sm_count) return few_by_group<T, O, 2, PIECES, 4>(ctx, a, st);
+            if (blocks >= 2 * ctx->sm_count) return few_by_group<T, O, 2, PIECES, 2>(ctx, a, st);
+        }
+    }
+    return a.tokens > 8 ? few_by_group<T, O, 2, PIECES, 1>(ctx, a, st) : few_by_group<T, O, 1, PIECES, 1>(ctx, a, st);
 }
 
 }  // namespace
@@ -547,7 +498,7 @@ llmc_status int4_stage(llmc_ctx* ctx, cudaStream_t st, const void* x, int dtype,
 
 llmc_status int4_few(llmc_ctx* ctx, cudaStream_t st, const w4::View& v, const void* x, int dtype, int64_t tokens, int64_t ldx,
                      int64_t xcols, const void* bias, void* y, int64_t ldy) {
-    FewArgs a{v, x, ldx, xcols, (int)tokens, bias, y, ldy, ctx->dflags + 2, ctx->wait_limit};
+    FewArgs a{v, x, ldx, xcols, (int)tokens, bias, y, ldy};
     if (dtype == LLMC_DTYPE_F32) return few_by_size<__nv_bfloat16, float, 3>(ctx, a, st);
     if (dtype == LLMC_DTYPE_BF16) return few_by_size<__nv_bfloat16, __nv_bfloat16, 1>(ctx, a, st);
     return few_by_size<__half, __half, 1>(ctx, a, st);

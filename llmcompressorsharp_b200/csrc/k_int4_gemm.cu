@@ -21,8 +21,8 @@
 // to fp32 registers.
 //
 // A persistent grid of CTA pairs (256 tokens x 256 columns, cta_group::2) or, for up to 128 tokens and for fp32,
-// single CTAs (128 x 128).  Per CTA: a TMA warp for the activations and one for the codes (a tile of eight records,
-// 128 x 128 weights, in one bulk copy), an MMA warp, epilogue warps, eight dequantising warps, a ring of
+// single CTAs (128 x 128).  Per CTA: a TMA warp for the activations and one for the codes (a tile of 128 x 128
+// weights in one bulk copy), an MMA warp, epilogue warps, eight dequantising warps, a ring of
 // STAGES x (32 KB activations + 32 KB weights) and one of CODE_STAGES tiles of codes, two accumulators in TMEM.
 // A stage is a whole tile, 128 of the contraction: the MMA thread's two waits and its commit take about 700 clocks,
 // which a stage of 64 (512 clocks of MMAs) did not cover (0.59 us a stage; see the figures at int4_gemm).
@@ -117,11 +117,11 @@ template <typename T, int PIECES> struct Scale {
 // Eight weights of a word in T: rounded once, or piece wp of their fp32 value (truncated, eight bits each, so the three
 // add up to it).
 template <typename T, int PIECES>
-__device__ __forceinline__ uint4 dequant(uint32_t word, const Scale<T, PIECES>& sc, int wp) {
+__device__ __forceinline__ uint4 dequant(uint32_t word, const Scale<T, PIECES>& sc, Bits bits, int wp) {
     uint32_t o[4];
 #pragma unroll
     for (int p = 0; p < 4; p++) {
-        const uint32_t v = int_pair<T>(word, p, sc.zz);
+        const uint32_t v = int_pair<T>(word, p, sc.zz, bits);
         if constexpr (PIECES == 1) {
             o[p] = bits2(__hfma2(as2<T>(v), sc.hi, __hmul2(as2<T>(v), sc.lo)));
         } else {
@@ -162,6 +162,7 @@ __global__ void __launch_bounds__(32 * (3 + (PIECES == 3 ? 8 : 4) + DQ_WARPS), 1
     uint64_t* cempty = cfull + CODE_STAGES;
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(cempty + CODE_STAGES);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+    uint2* slot = reinterpret_cast<uint2*>(tmem_slot + 2);
 
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
     const uint32_t rank = CG == 2 ? cluster_ctarank() : 0;
@@ -181,6 +182,7 @@ __global__ void __launch_bounds__(32 * (3 + (PIECES == 3 ? 8 : 4) + DQ_WARPS), 1
             mbar_init(&cempty[s], DQ_WARPS);
         }
         *abort_flag = 0;
+        put_bits<T>(slot);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == 0) {
@@ -416,6 +418,7 @@ __global__ void __launch_bounds__(32 * (3 + (PIECES == 3 ? 8 : 4) + DQ_WARPS), 1
         // ---- dequantising
         const int grp = (warp - 2 - EW) / 4, w = (warp - 2 - EW) % 4, ng = a.v.ng, t = lane & 3, r8 = row_of(lane);
         const int64_t lim = (DIR == 0 ? a.v.mp : a.v.kp) - 128;
+        const Bits bits = get_bits(slot);
         for (int un = worker; un < units && !*abort_flag; un += workers) {
             const Unit u = unit_at<CG>(a, un);
             // the last tile of a pair may reach past the padded weight: its columns are never stored
@@ -470,7 +473,7 @@ __global__ void __launch_bounds__(32 * (3 + (PIECES == 3 ? 8 : 4) + DQ_WARPS), 1
                     for (int c = 0; c < 4; c++) {
                         // K-major and MN-major alike: a box holds 64 layout columns of 128 rows, rows of 128 bytes
                         const int off = c / 2 * BOX_BYTES + (32 * w + 8 * i + r8) * 128 + (((4 * (c & 1) + t) ^ r8) << 4);
-                        *reinterpret_cast<uint4*>(b + off) = dequant<T, PIECES>(word[c], sc[i][c], wp);
+                        *reinterpret_cast<uint4*>(b + off) = dequant<T, PIECES>(word[c], sc[i][c], bits, wp);
                     }
                 }
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
