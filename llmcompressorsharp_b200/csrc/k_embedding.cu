@@ -12,6 +12,8 @@
 #include "ops.h"
 #include "tc_common.cuh"
 
+#include <atomic>
+
 namespace llmc {
 namespace {
 
@@ -93,9 +95,8 @@ constexpr int DIGIT = 9, BINS = 1 << DIGIT, BATCH = 8;
 constexpr int RUN = 32;
 
 struct Plan {           // the workspace of one gradient call
-    uint32_t *keys0, *keys1, *idx0, *idx1;
-    __host__ __device__ uint32_t* keys(int i) const { return i & 1 ? keys1 : keys0; }
-    __host__ __device__ uint32_t* idx(int i) const { return i & 1 ? idx1 : idx0; }
+    uint2 *pairs0, *pairs1;  // (token, id), sorted by id; the passes go from one to the other
+    __host__ __device__ uint2* pairs(int i) const { return i & 1 ? pairs1 : pairs0; }
     int2* span;         // [vocab] first and one past the last sorted position, (0, 0) for an absent row
     int* counts;        // pieces, cut rows
     int2* pieces;       // first position, tokens
@@ -107,8 +108,9 @@ int64_t max_pieces(int64_t tokens) { return 2 * (tokens / RUN) + 2; }
 
 // One cluster sorts: stable passes of up to nine bits, each warp counting and placing its own stretch of
 // tokens, the counts of a pass added up over the warps in shared memory and over the CTAs through it
-// (hardware cluster barriers, no spinning).  One launch in place of three per pass; a cluster reads and
-// writes the ids at a few hundred GB/s, little against the rows of the gradient themselves.  Padding tokens and ids outside the table sort last, as `vocab`.
+// (hardware cluster barriers, no spinning).  One launch in place of three per pass.  Bound by the scattered stores,
+// of which an SM does about one a clock, so token and id go out as one store of eight bytes and the cluster is as
+// large as it may be.  Padding tokens and ids outside the table sort last, as `vocab`.
 template <typename I>
 __global__ void __launch_bounds__(SORT_NT) sort_kernel(const I* ids, uint32_t tokens, int64_t vocab, int64_t padding, int passes,
                                                       int bits, Plan p, int* flag) {
@@ -127,23 +129,21 @@ __global__ void __launch_bounds__(SORT_NT) sort_kernel(const I* ids, uint32_t to
 
     // Each warp takes its stretch in batches of BATCH x 32 tokens, whose keys it loads at once: one latency a batch
     // instead of one for each 32 tokens (60 us became 20 for 65,536 of them).
-    uint32_t key[BATCH], idx[BATCH];
+    uint2 pair[BATCH];  // token, id
     bool bad = false;
-    auto load = [&](int pass, uint32_t i0, bool with_idx) {
+    auto load = [&](int pass, uint32_t i0) {
 #pragma unroll
         for (int q = 0; q < BATCH; q++) {
             const uint32_t i = i0 + q * 32 + lane;
-            key[q] = 0;
-            idx[q] = i;
+            pair[q] = make_uint2(i, 0);
             if (i >= last) continue;
             if (pass) {
-                key[q] = __ldcg(p.keys(pass + 1) + i);
-                if (with_idx) idx[q] = __ldcg(p.idx(pass + 1) + i);
+                pair[q] = __ldcg(p.pairs(pass + 1) + i);
             } else {
                 const int64_t id = (int64_t)ids[i];
                 const bool out = id < 0 || id >= vocab;
                 bad |= out;
-                key[q] = out || id == padding ? (uint32_t)vocab : (uint32_t)id;
+                pair[q].y = out || id == padding ? (uint32_t)vocab : (uint32_t)id;
             }
         }
     };
@@ -153,13 +153,13 @@ __global__ void __launch_bounds__(SORT_NT) sort_kernel(const I* ids, uint32_t to
         for (int b = threadIdx.x; b < SORT_WARPS * BINS; b += SORT_NT) hist[b] = 0;
         __syncthreads();
         for (uint32_t i = first; i < last; i += 32 * BATCH) {
-            load(pass, i, true);
+            load(pass, i);
 #pragma unroll
             for (int q = 0; q < BATCH; q++) {
                 const bool in = i + q * 32 + lane < last;
                 const unsigned live = __ballot_sync(0xffffffffu, in);
                 if (in) {
-                    const uint32_t d = (key[q] >> shift) & (bins - 1);
+                    const uint32_t d = (pair[q].y >> shift) & (bins - 1);
                     const unsigned peers = __match_any_sync(live, d);
                     if ((peers & ((1u << lane) - 1)) == 0) mine[d] += __popc(peers);
                 }
@@ -200,7 +200,7 @@ __global__ void __launch_bounds__(SORT_NT) sort_kernel(const I* ids, uint32_t to
         }
         __syncthreads();
         for (uint32_t i = first; i < last; i += 32 * BATCH) {
-            if (last - first > 32 * BATCH) load(pass, i, true);  // else the batch counted is the one to place
+            if (last - first > 32 * BATCH) load(pass, i);  // else the batch counted is the one to place
 #pragma unroll
             for (int q = 0; q < BATCH; q++) {
                 const bool in = i + q * 32 + lane < last;
@@ -208,11 +208,10 @@ __global__ void __launch_bounds__(SORT_NT) sort_kernel(const I* ids, uint32_t to
                 unsigned peers = 0;
                 uint32_t d = 0;
                 if (in) {
-                    d = (key[q] >> shift) & (bins - 1);
+                    d = (pair[q].y >> shift) & (bins - 1);
                     peers = __match_any_sync(live, d);
                     const uint32_t pos = base[d] + mine[d] + __popc(peers & ((1u << lane) - 1));
-                    __stcg(p.keys(pass) + pos, key[q]);
-                    __stcg(p.idx(pass) + pos, idx[q]);
+                    __stcg(p.pairs(pass) + pos, pair[q]);
                 }
                 __syncwarp();
                 if (in && (peers & ((1u << lane) - 1)) == 0) mine[d] += __popc(peers);
@@ -223,17 +222,18 @@ __global__ void __launch_bounds__(SORT_NT) sort_kernel(const I* ids, uint32_t to
         cluster_sync();  // the other CTAs read what this one placed, and its totals are read no more
     }
     if (bad) atomicOr(flag, 1);
-    const uint32_t* keys = p.keys(passes + 1);
+    const uint2* sorted = p.pairs(passes + 1);
+    const auto key_at = [&](uint32_t i) { return __ldcg(&sorted[i].y); };
     const uint32_t hop = ctas * SORT_NT;
     for (uint32_t i0 = rank * SORT_NT + threadIdx.x; i0 < tokens; i0 += hop * BATCH) {
-        uint32_t prev[BATCH], next[BATCH], far[BATCH];
+        uint32_t key[BATCH], prev[BATCH], next[BATCH], far[BATCH];
 #pragma unroll
         for (int q = 0; q < BATCH; q++) {
             const uint32_t i = i0 + q * hop;
-            key[q] = i < tokens ? __ldcg(keys + i) : (uint32_t)vocab;
-            prev[q] = i < tokens && i > 0 ? __ldcg(keys + i - 1) : ~0u;
-            next[q] = i + 1 < tokens ? __ldcg(keys + i + 1) : ~0u;
-            far[q] = i + RUN < tokens ? __ldcg(keys + i + RUN) : ~0u;
+            key[q] = i < tokens ? key_at(i) : (uint32_t)vocab;
+            prev[q] = i < tokens && i > 0 ? key_at(i - 1) : ~0u;
+            next[q] = i + 1 < tokens ? key_at(i + 1) : ~0u;
+            far[q] = i + RUN < tokens ? key_at(i + RUN) : ~0u;
         }
 #pragma unroll
         for (int q = 0; q < BATCH; q++) {
@@ -245,12 +245,12 @@ __global__ void __launch_bounds__(SORT_NT) sort_kernel(const I* ids, uint32_t to
             if (far[q] != key[q]) continue;
             // A run that is cut: its length by doubling and halving steps over the sorted keys.
             uint32_t lo = i + RUN, step = RUN;
-            while (lo + step < tokens && __ldcg(keys + lo + step) == key[q]) {
+            while (lo + step < tokens && key_at(lo + step) == key[q]) {
                 lo += step;
                 step *= 2;
             }
             for (; step > 0; step /= 2)
-                if (lo + step < tokens && __ldcg(keys + lo + step) == key[q]) lo += step;
+                if (lo + step < tokens && key_at(lo + step) == key[q]) lo += step;
             // Which slots a row gets is a race, but its pieces stand in order and are joined in order.
             const int n = (int)(lo + 1 - i), np = (n + RUN - 1) / RUN;
             const int at = atomicAdd(p.counts, np);
@@ -262,13 +262,13 @@ __global__ void __launch_bounds__(SORT_NT) sort_kernel(const I* ids, uint32_t to
 
 // ---- summing --------------------------------------------------------------------------------------
 template <typename T>
-__device__ __forceinline__ void sum_run(const T* dy, int64_t ld, const uint32_t* idx, int n, int j, float (&acc)[Vec<T>::N]) {
+__device__ __forceinline__ void sum_run(const T* dy, int64_t ld, const uint2* idx, int n, int j, float (&acc)[Vec<T>::N]) {
     constexpr int N = Vec<T>::N;
     int i = 0;
     for (; i + 4 <= n; i += 4) {  // four rows in flight, added in token order
         uint4 u[4];
 #pragma unroll
-        for (int q = 0; q < 4; q++) u[q] = __ldcs(reinterpret_cast<const uint4*>(dy + (int64_t)idx[i + q] * ld) + j);
+        for (int q = 0; q < 4; q++) u[q] = __ldcs(reinterpret_cast<const uint4*>(dy + (int64_t)idx[i + q].x * ld) + j);
 #pragma unroll
         for (int q = 0; q < 4; q++) {
             float f[N];
@@ -279,7 +279,7 @@ __device__ __forceinline__ void sum_run(const T* dy, int64_t ld, const uint32_t*
     }
     for (; i < n; i++) {
         float f[N];
-        unpack<T>(__ldcs(reinterpret_cast<const uint4*>(dy + (int64_t)idx[i] * ld) + j), f);
+        unpack<T>(__ldcs(reinterpret_cast<const uint4*>(dy + (int64_t)idx[i].x * ld) + j), f);
 #pragma unroll
         for (int k = 0; k < N; k++) acc[k] = __fadd_rn(acc[k], f[k]);
     }
@@ -288,7 +288,7 @@ __device__ __forceinline__ void sum_run(const T* dy, int64_t ld, const uint32_t*
 // The first `pblocks` blocks sum pieces, the others rows (L lanes per row): every row of the table is
 // written once, zeros where no token looked it up.  Bound by memory: dy read once, the table written once.
 template <typename T>
-__global__ void __launch_bounds__(256) sum_kernel(const T* dy, int64_t ld, const uint32_t* idx, Plan p, int64_t vocab,
+__global__ void __launch_bounds__(256) sum_kernel(const T* dy, int64_t ld, const uint2* idx, Plan p, int64_t vocab,
                                                  int64_t hidden, int L, int pblocks, float scale, T* out, int wide) {
     constexpr int N = Vec<T>::N;
     if ((int)blockIdx.x < pblocks) {
@@ -307,7 +307,7 @@ __global__ void __launch_bounds__(256) sum_kernel(const T* dy, int64_t ld, const
             } else {
                 for (int64_t j = threadIdx.x; j < hidden; j += 256) {
                     float acc = 0.f;
-                    for (int k = 0; k < s.y; k++) acc = __fadd_rn(acc, to_f<T>(dy[(int64_t)idx[s.x + k] * ld + j]));
+                    for (int k = 0; k < s.y; k++) acc = __fadd_rn(acc, to_f<T>(dy[(int64_t)idx[s.x + k].x * ld + j]));
                     part[j] = acc;
                 }
             }
@@ -329,7 +329,7 @@ __global__ void __launch_bounds__(256) sum_kernel(const T* dy, int64_t ld, const
         } else {
             for (int64_t j = lane; j < hidden; j += L) {
                 float acc = 0.f;
-                for (int k = 0; k < n; k++) acc = __fadd_rn(acc, to_f<T>(dy[(int64_t)idx[s.x + k] * ld + j]));
+                for (int k = 0; k < n; k++) acc = __fadd_rn(acc, to_f<T>(dy[(int64_t)idx[s.x + k].x * ld + j]));
                 out[v * hidden + j] = from_f<T>(__fmul_rn(acc, scale));
             }
         }
@@ -394,12 +394,34 @@ llmc_status lookup(llmc_ctx* ctx, cudaStream_t st, const void* table, int64_t ld
     return check_launch(ctx, "embedding");
 }
 
+// The sort's largest cluster: sixteen where the device places such a cluster, else the portable eight.
+int largest_cluster(int device, const void* fn, size_t sm) {
+    static std::atomic<int> known[64];
+    if (device < 0 || device >= 64) return 8;
+    int n = known[device].load(std::memory_order_relaxed);
+    if (n) return n;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(16);
+    cfg.blockDim = dim3(SORT_NT);
+    cfg.dynamicSmemBytes = sm;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = 16;
+    at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 1;
+    int clusters = 0;
+    const bool ok = cudaOccupancyMaxActiveClusters(&clusters, fn, &cfg) == cudaSuccess && clusters > 0;
+    if (!ok) cudaGetLastError();
+    n = ok ? 16 : 8;
+    known[device].store(n, std::memory_order_relaxed);
+    return n;
+}
+
 size_t carve(Plan& p, void* ws, int64_t tokens, int64_t vocab, int64_t hidden) {
     Carver c{(char*)ws};
-    p.keys0 = c.take<uint32_t>(tokens);
-    p.keys1 = c.take<uint32_t>(tokens);
-    p.idx0 = c.take<uint32_t>(tokens);
-    p.idx1 = c.take<uint32_t>(tokens);
+    p.pairs0 = c.take<uint2>(tokens);
+    p.pairs1 = c.take<uint2>(tokens);
     p.span = c.take<int2>(vocab);
     p.counts = c.take<int>(2);
     p.pieces = c.take<int2>(max_pieces(tokens));
@@ -419,7 +441,7 @@ llmc_status sums(llmc_ctx* ctx, cudaStream_t st, const void* dy, int64_t ld, int
     const int64_t rows = (vocab + per - 1) / per;
     const int64_t most = max_pieces(tokens);
     const int pblocks = tokens > RUN ? (int)(most < cap ? most : cap) : 0;
-    const uint32_t* idx = p.idx(passes + 1);
+    const uint2* idx = p.pairs(passes + 1);
     sum_kernel<T><<<(unsigned)(pblocks + (rows < 4 * cap ? rows : 4 * cap)), 256, 0, st>>>((const T*)dy, ld, idx, p, vocab, hidden, L, pblocks,
                                                                                   scale, (T*)out, wide);
     LLMC_TRY(check_launch(ctx, "embedding_grad_sum"));
@@ -453,11 +475,13 @@ llmc_status embedding_grad(llmc_ctx* ctx, cudaStream_t st, const void* ids, int 
     int width = 1;
     while ((1ll << width) <= vocab) width++;
     const int passes = (width + DIGIT - 1) / DIGIT, bits = (width + passes - 1) / passes;
-    int ctas = 1;  // about 4,096 tokens to a CTA, eight (the portable cluster) at most
-    while (ctas < 8 && (int64_t)ctas * 4096 < tokens) ctas *= 2;
     const size_t sm = (size_t)SORT_WARPS * BINS * sizeof(uint32_t);
     const void* fn = ids64 ? (const void*)sort_kernel<int64_t> : (const void*)sort_kernel<int32_t>;
     LLMC_CUDA_TRY(cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sm));
+    LLMC_CUDA_TRY(cudaFuncSetAttribute(fn, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+    const int most = largest_cluster(ctx->device, fn, sm);
+    int ctas = 1;  // about 2,048 tokens to a CTA
+    while (ctas < most && (int64_t)ctas * 2048 < tokens) ctas *= 2;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)ctas);
     cfg.blockDim = dim3(SORT_NT);
