@@ -154,8 +154,7 @@ def last_error() -> str:
 
 
 def call(name: str, *args) -> None:
-    lib = load()
-    st = getattr(lib, name)(*args)
+    st = getattr(_lib or load(), name)(*args)
     if st != 0:
         raise_for_status(st, f"{name}: {last_error()}")
 

@@ -9,8 +9,10 @@ This module supplies that caller:
 - ``LlamaShape`` presets for the model shapes the job is quoted on;
 - ``LlamaForCalibration``, a random-initialised LLaMA decoder with the usual module names
   (``model.layers.{i}.self_attn.q_proj`` ...), weights ~N(0, 0.02) from a seed, whose
-  forward is ordinary torch (cuBLAS GEMMs and SDPA): it only produces the activations that
-  reach the hooked Linear layers;
+  forward is ordinary torch (cuBLAS GEMMs and SDPA; on a CUDA device the embedding is the
+  library's): it only produces the activations that reach the hooked Linear layers;
+  ``load_compressed`` puts the packed weights a session leaves into it, to run the compressed
+  model on the same batches;
 - ``drive(model, batches)``, which runs the forward on each calibration batch and then hands
   the batch to ``CompressionSession.run``, so every modifier's OnBatch sees hooks that have
   already fired for that batch.
@@ -26,6 +28,8 @@ from dataclasses import dataclass
 
 import torch
 import torch.nn.functional as F
+
+from .packed import embedding, load_compressed
 
 
 @dataclass(frozen=True)
@@ -129,10 +133,17 @@ def _rope(x, cos, sin):
     return (x * cos + torch.cat((-x2, x1), dim=-1) * sin).to(x.dtype)
 
 
+class TokenEmbedding(torch.nn.Embedding):
+    """torch.nn.Embedding whose lookup, on a CUDA device, is the library's (the same values)."""
+
+    def forward(self, ids):
+        return embedding(ids, self.weight) if self.weight.is_cuda else super().forward(ids)
+
+
 class _Body(torch.nn.Module):
     def __init__(self, s: LlamaShape, dtype, device, g):
         super().__init__()
-        self.embed_tokens = torch.nn.Embedding(s.vocab, s.hidden, dtype=dtype, device=device)
+        self.embed_tokens = TokenEmbedding(s.vocab, s.hidden, dtype=dtype, device=device)
         with torch.no_grad():
             self.embed_tokens.weight.copy_((torch.randn(s.vocab, s.hidden, generator=g) * 0.02).to(dtype))
         self.embed_tokens.weight.requires_grad_(False)
@@ -171,6 +182,10 @@ class LlamaForCalibration(torch.nn.Module):
     def linear_modules(self) -> dict:
         """HF-style names -> Linear modules (``state.named_modules``)."""
         return {n: m for n, m in self.named_modules() if isinstance(m, torch.nn.Linear)}
+
+    def load_compressed(self, compressed: dict) -> list[str]:
+        """Puts packed modules in place of the compressed ones (``packed.load_compressed``)."""
+        return load_compressed(self, compressed)
 
     def linear_weights(self) -> dict:
         """``<module>.weight`` -> weight tensor (``state.named_weights``)."""

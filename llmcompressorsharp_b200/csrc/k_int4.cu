@@ -386,13 +386,15 @@ __global__ void __launch_bounds__(32 * FEW_WARPS) few_kernel(const FewArgs a) {
 template <typename O>
 __global__ void __launch_bounds__(256) join_kernel(const float* part, int splits, int64_t rows, int64_t cols, const O* bias,
                                                   O* out, int64_t ldo) {
-    const int64_t total = rows * cols;
-    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
+    const int64_t c = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (c >= cols) return;
+    const float b = bias ? to_f<O>(bias[c]) : 0.f;
+    for (int64_t r = blockIdx.y; r < rows; r += gridDim.y) {
         float s = 0.f;
-        for (int p = 0; p < splits; p++) s += part[p * total + i];
-        const int64_t c = i % cols;
-        if (bias) s += to_f<O>(bias[c]);
-        out[i / cols * ldo + c] = from_f<O>(s);
+        const float* p = part + r * cols + c;
+#pragma unroll 4
+        for (int k = 0; k < splits; k++) s += p[k * rows * cols];
+        out[r * ldo + c] = from_f<O>(s + b);
     }
 }
 
@@ -506,7 +508,8 @@ llmc_status int4_few(llmc_ctx* ctx, cudaStream_t st, const w4::View& v, const vo
 
 llmc_status int4_join(llmc_ctx* ctx, cudaStream_t st, const float* part, int splits, int64_t rows, int64_t cols, const void* bias,
                       void* out, int dtype, int64_t ldo) {
-    const int grid = grid_n(ctx, rows * cols);
+    const int64_t wide = (cols + 255) / 256, most = 16 * (int64_t)ctx->sm_count / wide + 1;
+    const dim3 grid((unsigned)wide, (unsigned)(rows < most ? rows : most));
     if (dtype == LLMC_DTYPE_F32)
         join_kernel<float><<<grid, 256, 0, st>>>(part, splits, rows, cols, (const float*)bias, (float*)out, ldo);
     else if (dtype == LLMC_DTYPE_BF16)

@@ -126,7 +126,9 @@ __device__ __forceinline__ uint4 dequant(uint32_t word, const Scale<T, PIECES>& 
             o[p] = bits2(__hfma2(as2<T>(v), sc.hi, __hmul2(as2<T>(v), sc.lo)));
         } else {
             float w0 = __fmul_rn(__uint_as_float(v << 16), sc.s), w1 = __fmul_rn(__uint_as_float(v & 0xFFFF0000u), sc.s);
-            for (int q = 0; q < wp; q++) {
+#pragma unroll
+            for (int q = 0; q < 2; q++) {
+                if (q >= wp) continue;
                 w0 = __fsub_rn(w0, __uint_as_float(__float_as_uint(w0) & 0xFFFF0000u));
                 w1 = __fsub_rn(w1, __uint_as_float(__float_as_uint(w1) & 0xFFFF0000u));
             }
@@ -308,63 +310,62 @@ __global__ void __launch_bounds__(32 * (3 + (PIECES == 3 ? 8 : 4) + DQ_WARPS), 1
         for (int un = worker; un < units && !*abort_flag; un += workers) {
             const Unit u = unit_at<CG>(a, un);
             const int64_t tok = u.m0 + rank * 128 + q * 32 + lane;
-            auto emit = [&](const float (&v)[32], int c0) {  // columns n0 + c0 .. + 31 of this thread's token
-                if (tok >= a.tokens) return;
+            // Columns n0 + c0 .. + 31 of this warp's 32 tokens, one token to a thread.
+            auto emit = [&](float (&v)[32], int c0) {
+                constexpr bool HALF = Num<T>::MAGIC == Num<__half>::MAGIC;
                 const int64_t col0 = u.n0 + c0;
-                float o[32];
-#pragma unroll
-                for (int i = 0; i < 32; i++) {
-                    o[i] = v[i];
-                    if constexpr (Num<T>::MAGIC == Num<__half>::MAGIC) {
-                        const int64_t col = col0 + i;
-                        if (DIR == 0) {
-                            if (col < a.v.rows) o[i] *= pow2(__ldg(a.v.exps + col));
-                        } else {
-                            if (col < a.v.kp) o[i] *= pow2(__ldg(a.v.exps + a.v.mp + col / TILE * a.v.ng + slot_of((int)(col % TILE) / 32, a.v.ng)));
-                        }
-                    }
-                }
-                const bool part = a.splits > 1;
-                float* prow = a.part + ((int64_t)u.split * a.tokens + tok) * a.ocols;
-                O* row = reinterpret_cast<O*>(a.out) + tok * a.ldo;
-                const bool mapped = DIR == 1 && !a.v.identity;
-                if (!part && a.wide && !mapped && col0 + 32 <= a.ocols) {
-                    constexpr int N = 16 / (int)sizeof(O);
-#pragma unroll
-                    for (int i = 0; i < 32; i += N) {
-                        union { O h[N]; uint4 u4; } x;
-#pragma unroll
-                        for (int j = 0; j < N; j++) {
-                            float f = o[i + j];
-                            if (a.bias) f += to_f<O>(reinterpret_cast<const O*>(a.bias)[col0 + i + j]);
-                            x.h[j] = from_f<O>(f);
-                        }
-                        *reinterpret_cast<uint4*>(row + col0 + i) = x.u4;
-                    }
-                    return;
-                }
-                if (part && !mapped && a.ocols % 4 == 0 && col0 + 32 <= a.ocols) {
-#pragma unroll
-                    for (int i = 0; i < 32; i += 4)
-                        *reinterpret_cast<float4*>(prow + col0 + i) = make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
-                    return;
-                }
-#pragma unroll
-                for (int i = 0; i < 32; i++) {
-                    int64_t col = col0 + i;
-                    if (mapped) {
-                        if (col >= a.v.kp) continue;
-                        col = column_of((int)col, a.v.gs, a.v.gsv, a.v.groups, a.v.cols);
-                        if (col < 0) continue;
-                    }
-                    if (col >= a.ocols) continue;
+                const bool part = a.splits > 1, mapped = DIR == 1 && !a.v.identity;
+                if (!HALF && !mapped && !a.bias && (part ? a.ocols % 4 == 0 : a.wide) && col0 + 32 <= a.ocols) {
+                    // 16 bytes at a time along the thread's own row
+                    if (tok >= a.tokens) return;
                     if (part) {
-                        prow[col] = o[i];
+                        float* row = a.part + ((int64_t)u.split * a.tokens + tok) * a.ocols + col0;
+#pragma unroll
+                        for (int i = 0; i < 32; i += 4) *reinterpret_cast<float4*>(row + i) = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
                     } else {
-                        float f = o[i];
-                        if (a.bias) f += to_f<O>(reinterpret_cast<const O*>(a.bias)[col]);
-                        row[col] = from_f<O>(f);
+                        constexpr int N = 16 / (int)sizeof(O);
+                        O* row = reinterpret_cast<O*>(a.out) + tok * a.ldo + col0;
+#pragma unroll
+                        for (int i = 0; i < 32; i += N) {
+                            union { O h[N]; uint4 u4; } x;
+#pragma unroll
+                            for (int j = 0; j < N; j++) x.h[j] = from_f<O>(v[i + j]);
+                            *reinterpret_cast<uint4*>(row + i) = x.u4;
+                        }
                     }
+                    return;
+                }
+                // Otherwise the block is transposed in registers, so that a thread has one column (its bias, its exponent,
+                // where it goes) and a store is 32 neighbours of a row; element by element along rows, a product with
+                // an odd number of columns spent 27 us of 36 in its stores.
+#pragma unroll
+                for (int s = 16; s > 0; s >>= 1)
+#pragma unroll
+                    for (int i = 0; i < 32; i++) {
+                        if (i & s) continue;
+                        const bool hi = lane & s;
+                        const float y = __shfl_xor_sync(0xffffffffu, hi ? v[i] : v[i | s], s);
+                        if (hi) v[i] = y;
+                        else v[i | s] = y;
+                    }
+                int64_t col = col0 + lane;
+                float f = 1.f;
+                if (HALF) {
+                    if (DIR == 0) f = col < a.v.rows ? pow2(__ldg(a.v.exps + col)) : 1.f;
+                    else f = col < a.v.kp ? pow2(__ldg(a.v.exps + a.v.mp + col / TILE * a.v.ng + slot_of((int)(col % TILE) / 32, a.v.ng))) : 1.f;
+                }
+                if (mapped) col = col < a.v.kp ? column_of((int)col, a.v.gs, a.v.gsv, a.v.groups, a.v.cols) : -1;
+                if (col < 0 || col >= a.ocols) return;
+                const float bias = a.bias ? to_f<O>(reinterpret_cast<const O*>(a.bias)[col]) : 0.f;
+                const int64_t tok0 = tok - lane;
+                const int n = (int)min((int64_t)32, a.tokens - tok0);
+                float* pcol = a.part + ((int64_t)u.split * a.tokens + tok0) * a.ocols + col;
+                O* ocol = reinterpret_cast<O*>(a.out) + tok0 * a.ldo + col;
+#pragma unroll
+                for (int r = 0; r < 32; r++) {
+                    if (r >= n) break;
+                    if (part) pcol[r * a.ocols] = v[r] * f;
+                    else ocol[r * a.ldo] = from_f<O>(fmaf(v[r], f, bias));
                 }
             };
             const int chunks = FOLDS ? (u.kt1 - u.kt0 + FOLD - 1) / FOLD : 1;
@@ -615,13 +616,15 @@ llmc_status launch(llmc_ctx* ctx, cudaStream_t st, const CUtensorMap& map, GemmI
 // CTAs per tile for a product of this many tokens and columns.
 int int4_gemm_cg(int dtype, int64_t tokens, int64_t cols) { return dtype != LLMC_DTYPE_F32 && tokens > 128 && cols > 128 ? 2 : 1; }
 
-// Splits of the contraction: enough to give every worker a tile, two tiles of 128 to a split at least.
+// Splits of the contraction: enough to give every worker a tile, two tiles of 128 to a split at least (one in fp32,
+// where a tile is six products).
 int int4_gemm_splits(const llmc_ctx* ctx, int dtype, int64_t tokens, int64_t cols, int64_t contraction) {
     const int cg = int4_gemm_cg(dtype, tokens, cols);
     const int64_t tile = 128 * cg, tiles = ((tokens + tile - 1) / tile) * ((cols + tile - 1) / tile);
     const int64_t kt = contraction / TILE, workers = persistent_sms(ctx) / cg;
     int64_t s = workers / tiles;
-    if (s > kt / 2) s = kt / 2;
+    const int64_t most = dtype == LLMC_DTYPE_F32 ? kt : kt / 2;
+    if (s > most) s = most;
     if (s > 32) s = 32;
     if (s < 1) s = 1;
     const int64_t per = (kt + s - 1) / s;

@@ -19,6 +19,7 @@ from __future__ import annotations
 import ctypes as C
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from . import _lib
 from ._device import target_device, to_device
@@ -55,7 +56,9 @@ class Int4Weight:
     ``codes`` are as ``rtn_quantize`` and the GPTQ calls write them for num_bits <= 4:
     (q - zp) & 0xF, two per byte, the even column in the high nibble (Int4PackedTensor.cs:47-69).
     They are laid out anew (and rounded up to 128 rows and columns); the tensors passed in are not
-    kept.  Groups have at least 16 columns.  The weight is constant: its scales take no gradient."""
+    kept.  Groups have at least 16 columns.  The weight is constant: its scales take no gradient.  It
+    stays on its device (a module's ``to`` does not move it) and is in no ``state_dict``; it can be
+    copied and pickled."""
 
     def __init__(self, codes: torch.Tensor, scales: torch.Tensor, zero_points: torch.Tensor | None, cols: int,
                  strategy: str = "group", group_size: int = 128, symmetric: bool = True, num_bits: int = 4):
@@ -90,12 +93,23 @@ class Int4Weight:
         z = to_device(zero_points.detach(), self.device, torch.int32) if not symmetric else None
         self.packed = torch.empty(size.value, dtype=torch.uint8, device=self.device)
         self.exps = torch.empty(exps.value, dtype=torch.int32, device=self.device)
-        self._c = _lib.Int4WeightC(self.packed.data_ptr(), self.exps.data_ptr(), rows, int(cols), group)
+        self._bind()
+        _lib.call("llmc_int4_layout", self._ctx, _lib.stream(self._index), _lib.ptr(c), c.shape[1], _lib.ptr(s), _lib.ptr(z),
+                  _lib.STRATEGY[strategy], int(symmetric), self._ref)
+
+    def _bind(self):
+        self._c = _lib.Int4WeightC(self.packed.data_ptr(), self.exps.data_ptr(), *self.shape, self.group_size)
         self._ref = C.byref(self._c)
         self._ctx, self._index = _lib.ctx_handle(self.device.index), self.device.index
         self._need: dict = {}
-        _lib.call("llmc_int4_layout", self._ctx, _lib.stream(self._index), _lib.ptr(c), c.shape[1], _lib.ptr(s), _lib.ptr(z),
-                  _lib.STRATEGY[strategy], int(symmetric), self._ref)
+
+    def __getstate__(self):
+        return {k: v for k, v in self.__dict__.items() if k not in ("_c", "_ref", "_ctx", "_index", "_need")}
+
+    def __setstate__(self, state):
+        self.__dict__.update(state)
+        self.device = self.packed.device
+        self._bind()
 
     @staticmethod
     def from_entry(entry: dict, cols: int) -> "Int4Weight":
@@ -155,13 +169,27 @@ class Int4Weight:
         return out
 
 
+_needs: dict = {}  # (call, device, sizes) -> bytes of scratch
+
+
+def _scratch(fn: str, index: int, device, *sizes) -> torch.Tensor:
+    """Scratch tensor of a call whose need depends on its sizes alone."""
+    key = (fn, index, sizes)
+    need = _needs.get(key)
+    if need is None:
+        v = _lib.I64()
+        _lib.call(fn, _lib.ctx_handle(index), *sizes, C.byref(v))
+        if len(_needs) >= 256:
+            _needs.clear()
+        need = _needs[key] = v.value
+    return torch.empty(need, dtype=torch.uint8, device=device)
+
+
 def _col_sum(x2: torch.Tensor) -> torch.Tensor:
     index = x2.device.index
     ctx = _lib.ctx_handle(index)
     rows, cols = x2.shape
-    need = _lib.I64()
-    _lib.call("llmc_col_sum_workspace", ctx, rows, cols, C.byref(need))
-    ws = torch.empty(need.value, dtype=torch.uint8, device=x2.device)
+    ws = _scratch("llmc_col_sum_workspace", index, x2.device, rows, cols)
     out = torch.empty(cols, dtype=x2.dtype, device=x2.device)
     _lib.call("llmc_col_sum", ctx, _lib.stream(index), x2.data_ptr(), _DTYPES[x2.dtype], rows, cols, _pitch(x2), out.data_ptr(),
               ws.data_ptr(), ws.numel())
@@ -175,6 +203,7 @@ class _Int4LinearFn(torch.autograd.Function):
         return weight._product(_rows(x, weight.shape[1]), bias, False).reshape(*x.shape[:-1], weight.shape[0])
 
     @staticmethod
+    @once_differentiable
     def backward(ctx_, dy):
         w = ctx_.weight
         d2 = _rows(dy, w.shape[0])
@@ -229,6 +258,7 @@ class _EmbeddingFn(torch.autograd.Function):
         return _lookup(ids.reshape(-1), table, scale).reshape(*ids.shape, table.shape[1])
 
     @staticmethod
+    @once_differentiable
     def backward(ctx_, dy):
         (ids,) = ctx_.saved_tensors
         vocab, hidden = ctx_.shape
@@ -236,9 +266,7 @@ class _EmbeddingFn(torch.autograd.Function):
         flat = ids.reshape(-1)
         index = dy.device.index
         ctx = _lib.ctx_handle(index)
-        need = _lib.I64()
-        _lib.call("llmc_embedding_grad_workspace", ctx, flat.numel(), vocab, hidden, C.byref(need))
-        ws = torch.empty(need.value, dtype=torch.uint8, device=dy.device)
+        ws = _scratch("llmc_embedding_grad_workspace", index, dy.device, flat.numel(), vocab, hidden)
         out = torch.empty(vocab, hidden, dtype=dy.dtype, device=dy.device)
         _lib.call("llmc_embedding_grad", ctx, _lib.stream(index), flat.data_ptr(), int(flat.dtype == torch.int64), flat.numel(),
                   d2.data_ptr(), _DTYPES[dy.dtype], _pitch(d2), vocab, hidden, ctx_.scale, ctx_.padding, out.data_ptr(),
