@@ -21,8 +21,14 @@ struct DeviceScope {
 };
 
 constexpr int64_t MAX_DIM = (int64_t)1 << 30;     // rows, columns, tokens
-// Tokens that go to the few-row kernel; it takes 16 at a time, and the codes anew for each 16.
-constexpr int64_t FEW_16 = 16, FEW_F32 = 128;
+// Products that go to the few-row kernel, which reads the codes anew for each 16 tokens: up to 16 tokens, and more while
+// tokens / 16 x weights stays below what it passes the tensor-core kernel at.  That one takes about 9 us for any
+// product and as long for 17 tokens as for 128.  576 -> 1536 in bf16, 128 tokens: 9 us here, 13 there; 4096 -> 4096, 32: 15
+// and 14.5, 64: 23 and 16.  fp32 costs six products there and three here: 4096 -> 4096, 128: 86 here.
+bool few_rows(bool f32, int64_t tokens, int64_t rows, int64_t cols) {
+    if (tokens <= 16) return true;
+    return tokens <= (f32 ? 256 : 128) && (tokens + 15) / 16 * rows * cols <= (int64_t)1 << (f32 ? 27 : 25);
+}
 
 llmc_status check_sizes(int64_t rows, int64_t cols, int64_t gs) {
     if (rows <= 0 || cols <= 0) return fail(LLMC_ERR_SHAPE, "a packed weight needs positive sizes (got %lld x %lld)", (long long)rows, (long long)cols);
@@ -81,7 +87,7 @@ struct LinearPlan {
 LinearPlan plan_linear(const llmc_ctx* ctx, const w4::View& v, int dir, const void* a, int dtype, int64_t tokens, int64_t ld) {
     LinearPlan p{};
     const bool f32 = dtype == LLMC_DTYPE_F32;
-    p.few = dir == 0 && tokens <= (f32 ? FEW_F32 : FEW_16);
+    p.few = dir == 0 && few_rows(f32, tokens, v.rows, v.cols);
     // 16-byte rows are what both kernels load; the few-row one reads whole vectors of eight columns, TMA
     // fills what is past the last column.  fp32 is read in bf16 pieces, other groups in the layout's columns.
     p.stage = f32 || (uintptr_t)a % 16 != 0 || (ld % 8 != 0) || (dir == 0 && !v.identity) || (p.few && v.cols % 8 != 0);

@@ -336,26 +336,42 @@ __global__ void __launch_bounds__(256) sum_kernel(const T* dy, int64_t ld, const
     }
 }
 
-// Rows that were cut: 32 columns per item, sixteen warps each adding every sixteenth piece, then their sums.
+// Rows that were cut, 512 columns to an item.  A thread adds a column's pieces in order, or, where they are many,
+// sixteen warps add every sixteenth piece of 32 columns at a time and then their sums.
 template <typename T>
 __global__ void __launch_bounds__(512) join_cut_kernel(Plan p, int64_t hidden, float scale, T* out) {
     __shared__ float sm[16][33];
     const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
-    const int64_t slabs = (hidden + 31) / 32, items = (int64_t)p.counts[1] * slabs;
+    const int64_t slabs = (hidden + 511) / 512, items = (int64_t)p.counts[1] * slabs;
     for (int64_t i = blockIdx.x; i < items; i += gridDim.x) {
         const int4 c = p.cut[i / slabs];
-        const int64_t col = i % slabs * 32 + lane;
-        float s = 0.f;
-        if (col < hidden)
-            for (int k = warp; k < c.z; k += 16) s = __fadd_rn(s, p.partial[(int64_t)(c.y + k) * hidden + col]);
-        sm[warp][lane] = s;
-        __syncthreads();
-        if (warp == 0 && col < hidden) {
-#pragma unroll
-            for (int w = 1; w < 16; w++) s = __fadd_rn(s, sm[w][lane]);
-            out[(int64_t)c.x * hidden + col] = from_f<T>(__fmul_rn(s, scale));
+        const int64_t col0 = i % slabs * 512;
+        const float* part = p.partial + (int64_t)c.y * hidden;
+        T* row = out + (int64_t)c.x * hidden;
+        if (c.z <= 64) {
+            const int64_t col = col0 + threadIdx.x;
+            float s = 0.f;
+            if (col < hidden) {
+#pragma unroll 8
+                for (int k = 0; k < c.z; k++) s = __fadd_rn(s, part[k * hidden + col]);
+                row[col] = from_f<T>(__fmul_rn(s, scale));
+            }
+            continue;
         }
-        __syncthreads();
+        for (int64_t col = col0 + lane; col - lane < min(hidden, col0 + 512); col += 32) {
+            float s = 0.f;
+            if (col < hidden)
+#pragma unroll 8
+                for (int k = warp; k < c.z; k += 16) s = __fadd_rn(s, part[k * hidden + col]);
+            sm[warp][lane] = s;
+            __syncthreads();
+            if (warp == 0 && col < hidden) {
+#pragma unroll
+                for (int w = 1; w < 16; w++) s = __fadd_rn(s, sm[w][lane]);
+                row[col] = from_f<T>(__fmul_rn(s, scale));
+            }
+            __syncthreads();
+        }
     }
 }
 

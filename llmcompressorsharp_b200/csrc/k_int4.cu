@@ -7,6 +7,8 @@
 #include "ops.h"
 #include "tc_common.cuh"
 
+#include <atomic>
+
 namespace llmc {
 namespace {
 
@@ -229,7 +231,9 @@ struct FewArgs {
 };
 
 constexpr int FEW_WARPS = 8;  // per CTA at most
-__host__ __device__ constexpr int few_stages(int rb) { return rb == 1 ? 5 : 3; }
+// Tiles of the columns to a step and steps to a ring: what shared memory holds with sixteen tokens.
+__host__ __device__ constexpr int few_tiles(int nt, int rb) { return nt == 1 && rb == 1 ? 2 : 1; }
+__host__ __device__ constexpr int few_stages(int nt, int rb) { return nt == 2 && rb == 1 ? 5 : 3; }
 
 __device__ __forceinline__ void copy16(void* dst, const void* src, int bytes) {  // bytes < 16: zeros for the rest
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(tc::smem_u32(dst)), "l"(src), "r"(bytes) : "memory");
@@ -239,15 +243,16 @@ __device__ __forceinline__ void copy16(void* dst, const void* src, int bytes) { 
 // dequantised fragment serves eight tokens and a single token costs no more than the codes.  Codes enter as
 // the exact integers u - z; the fp32 sum of a group is multiplied by its scale (4 / NG granules of 32 columns per
 // group sum), so x and W are never rounded.  Columns of the MMA that stand for no token repeat the last one's x.
-// A CTA holds RB records' rows (16 RB) and 8 NT tokens; its warps take the 128-column steps in turn and add their sums
-// in shared memory, in warp order.  Each warp keeps a ring of STAGES steps in flight, the records and the 256 bytes
-// of each token's x (XS), by 16-byte asynchronous copies that it waits for by itself.  The three pieces of fp32 x would
-// take most of the ring and are read through L1, which row blocks of few columns share.
+// A CTA holds RB records' rows (16 RB) and 8 NT tokens; its warps take steps of FEW_TILES 128-column tiles in turn and
+// add their sums in shared memory, in warp order.  Each warp keeps a ring of STAGES steps, the records and the 256 bytes
+// a tile of each token's x (XS), by 16-byte asynchronous copies that it waits for by itself.  The three pieces of fp32
+// x would take most of the ring and are read through L1, which row blocks of few columns share.
 // What bounds it is the instructions: at the HBM's rate an SM has 43 clocks for a record, 172 issue slots, of which
-// turning its codes into numbers takes 88.
+// turning its codes into numbers takes 88 and the rest of its arithmetic 26; loops, copies and waits took 110 more
+// with a tile to a step.
 template <typename T, typename O, int NT, int PIECES, int NG, int RB>
 __global__ void __launch_bounds__(32 * FEW_WARPS) few_kernel(const FewArgs a) {
-    constexpr int REC = 1024 + 80 * NG, FL = 4 / NG, SUMS = 8 * NT * ROWS * RB, STAGES = few_stages(RB);
+    constexpr int REC = 1024 + 80 * NG, FL = 4 / NG, SUMS = 8 * NT * ROWS * RB, STAGES = few_stages(NT, RB), FEW_TILES = few_tiles(NT, RB);
     constexpr bool XS = PIECES == 1;
     extern __shared__ __align__(128) uint8_t smem[];  // int_pair's operands, rings; afterwards [warps][8 NT][16 RB] of sums
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, warps = blockDim.x / 32;
@@ -255,42 +260,50 @@ __global__ void __launch_bounds__(32 * FEW_WARPS) few_kernel(const FewArgs a) {
     const int tok0 = blockIdx.y * 8 * NT, toks = min(8 * NT, a.tokens - tok0);
     const int64_t row0 = (int64_t)blockIdx.x * (ROWS * RB);
     const int ktiles = (int)(a.v.kp / TILE);
-    const int room = RB * REC + (XS ? toks * 256 : 0);
+    const int xrow = FEW_TILES * 256, xat0 = FEW_TILES * RB * REC, room = xat0 + (XS ? toks * xrow : 0);
     uint8_t* ring = smem + 16 + warp * STAGES * room;
     if (threadIdx.x == 0) put_bits<T>(reinterpret_cast<uint2*>(smem));
     __syncthreads();
     const Bits bits = get_bits(reinterpret_cast<const uint2*>(smem));
 
-    int fkt = warp;  // the step to fetch next
-    const uint8_t* src = a.v.packed + record_at(a.v, row0, warp) + lane * 16;
-    const T* xsrc = reinterpret_cast<const T*>(a.x) + (int64_t)(tok0 + lane / 16) * a.ldx + warp * TILE + lane % 16 * 8;
+    constexpr int64_t TILE_BYTES = TILE / ROWS * REC;
+    const int hop = warps * FEW_TILES;  // tiles from one of this warp's steps to its next
+    int fkt = warp * FEW_TILES;         // the step to fetch next
+    const uint8_t* src = a.v.packed + record_at(a.v, row0, fkt) + lane * 16;
+    const T* xsrc = reinterpret_cast<const T*>(a.x) + (int64_t)(tok0 + lane / (16 * FEW_TILES)) * a.ldx + fkt * TILE + lane % (16 * FEW_TILES) * 8;
     auto fetch = [&](uint8_t* stage) {
         if (fkt < ktiles) {
             uint8_t* dst = stage + lane * 16;
 #pragma unroll
-            for (int i = 0; i < RB * REC / 512; i++) copy16(dst + i * 512, src + i * 512, 16);
-            if (lane < RB * REC % 512 / 16) copy16(dst + RB * REC / 512 * 512, src + RB * REC / 512 * 512, 16);
-            if (XS) {
-                // two tokens' 256 bytes to a copy; zeros past the last column
-                const bool in = fkt * TILE + lane % 16 * 8 < a.xcols;
-                const T* xr = in ? xsrc : reinterpret_cast<const T*>(a.x);
-                const int64_t two = in ? 2 * a.ldx : 0;
-                for (int r = lane / 16; r < toks; r += 2, xr += two) copy16(stage + RB * REC + r * 256 + lane % 16 * 16, xr, in ? 16 : 0);
+            for (int k = 0; k < FEW_TILES; k++) {
+                if (k > 0 && fkt + k >= ktiles) break;
+#pragma unroll
+                for (int i = 0; i < RB * REC / 512; i++) copy16(dst + k * RB * REC + i * 512, src + k * TILE_BYTES + i * 512, 16);
+                if (lane < RB * REC % 512 / 16)
+                    copy16(dst + k * RB * REC + RB * REC / 512 * 512, src + k * TILE_BYTES + RB * REC / 512 * 512, 16);
             }
-            fkt += warps;
-            src += (int64_t)warps * (TILE / ROWS) * REC;
-            xsrc += warps * TILE;
+            if (XS) {  // zeros past the last column
+                constexpr int EACH = 2 / FEW_TILES;  // tokens to a copy: a token's x of a step is 16 lanes' or 32
+                const bool in = fkt * TILE + lane % (16 * FEW_TILES) * 8 < a.xcols;
+                const T* xr = in ? xsrc : reinterpret_cast<const T*>(a.x);
+                const int64_t next = in ? EACH * a.ldx : 0;
+                for (int r = lane / (16 * FEW_TILES); r < toks; r += EACH, xr += next)
+                    copy16(stage + xat0 + r * xrow + lane % (16 * FEW_TILES) * 16, xr, in ? 16 : 0);
+            }
+            fkt += hop;
+            src += hop * TILE_BYTES;
+            xsrc += hop * TILE;
         }
         asm volatile("cp.async.commit_group;" ::: "memory");
     };
 #pragma unroll
     for (int s = 0; s < STAGES - 1; s++) fetch(ring + s * room);
 
-    int xat[NT];  // this lane's token of each eight in a stage, or (in elements) in x
+    int xat[NT];  // this lane's token of each eight: its x in a stage, or its number
 #pragma unroll
-    for (int n = 0; n < NT; n++) xat[n] = min(n * 8 + g, toks - 1);
+    for (int n = 0; n < NT; n++) xat[n] = XS ? xat0 + min(n * 8 + g, toks - 1) * xrow + t * 16 : min(n * 8 + g, toks - 1);
     auto load_x = [&](const uint8_t* stage, int kt, int c, int n, int p) {
-        if (XS) return *reinterpret_cast<const uint4*>(stage + RB * REC + xat[n] * 256 + t * 16 + c * 64);
+        if (XS) return *reinterpret_cast<const uint4*>(stage + xat[n] + c * 64);
         const int k = kt * TILE + 32 * c + 8 * t;
         if (k >= a.xcols) return make_uint4(0, 0, 0, 0);
         return __ldg(reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(a.x) + ((int64_t)p * a.tokens + tok0 + xat[n]) * a.ldx + k));
@@ -302,61 +315,64 @@ __global__ void __launch_bounds__(32 * FEW_WARPS) few_kernel(const FewArgs a) {
         for (int n = 0; n < NT; n++)
 #pragma unroll
             for (int j = 0; j < 4; j++) acc[r][n][j] = 0.f;
-    int at = 0, to = (STAGES - 1) * room;  // the stages to multiply and to fill
-    for (int kt = warp; kt < ktiles; kt += warps) {
+    int at = 0, free = (STAGES - 1) * room;  // the stages to multiply and to fill
+    for (int kt0 = warp * FEW_TILES; kt0 < ktiles; kt0 += hop) {
         asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 2) : "memory");
         __syncwarp();
-        fetch(ring + to);
-        const uint8_t* stage = ring + at;
+        fetch(ring + free);
+        free = at;
+        const uint8_t *rec = ring + at, *xstage = rec;
         at = at == (STAGES - 1) * room ? 0 : at + room;
-        to = to == (STAGES - 1) * room ? 0 : to + room;
-        uint32_t w[RB][2][4], zz[RB][2][NG];
-        float sc[RB][2][NG];
+#pragma unroll 1
+        for (int kt = kt0; kt < min(ktiles, kt0 + FEW_TILES); kt++, rec += RB * REC, xstage += 256) {
+            uint32_t w[RB][2][4], zz[RB][2][NG];
+            float sc[RB][2][NG];
 #pragma unroll
-        for (int r = 0; r < RB; r++)
+            for (int r = 0; r < RB; r++)
 #pragma unroll
-            for (int h = 0; h < 2; h++) {
-                const uint8_t* q = stage + r * REC;
-                const int row = g + 8 * h;
-                const uint4 u = *reinterpret_cast<const uint4*>(q + row * 64 + t * 16);
-                w[r][h][0] = u.x;
-                w[r][h][1] = u.y;
-                w[r][h][2] = u.z;
-                w[r][h][3] = u.w;
+                for (int h = 0; h < 2; h++) {
+                    const uint8_t* q = rec + r * REC;
+                    const int row = g + 8 * h;
+                    const uint4 u = *reinterpret_cast<const uint4*>(q + row * 64 + t * 16);
+                    w[r][h][0] = u.x;
+                    w[r][h][1] = u.y;
+                    w[r][h][2] = u.z;
+                    w[r][h][3] = u.w;
 #pragma unroll
-                for (int j = 0; j < NG; j++) {
-                    sc[r][h][j] = reinterpret_cast<const float*>(q + 1024)[row * NG + j];
-                    zz[r][h][j] = q[1024 + 64 * NG + row * NG + j] * 0x10001u + bits.magic;
+                    for (int j = 0; j < NG; j++) {
+                        sc[r][h][j] = reinterpret_cast<const float*>(q + 1024)[row * NG + j];
+                        zz[r][h][j] = q[1024 + 64 * NG + row * NG + j] * 0x10001u + bits.magic;
+                    }
                 }
-            }
-        float d[RB][NT][4];
+            float d[RB][NT][4];
 #pragma unroll
-        for (int c = 0; c < 4; c++) {
-            const int j = c / FL;
-            uint4 b[NT][PIECES];
-#pragma unroll
-            for (int n = 0; n < NT; n++)
-#pragma unroll
-                for (int p = 0; p < PIECES; p++) b[n][p] = load_x(stage, kt, c, n, p);
-#pragma unroll
-            for (int r = 0; r < RB; r++) {
-                uint32_t f[2][4];
-#pragma unroll
-                for (int h = 0; h < 2; h++)
-#pragma unroll
-                    for (int k = 0; k < 4; k++) f[h][k] = int_pair<T>(w[r][k & 1][c], 2 * h + k / 2, zz[r][k & 1][j], bits);
+            for (int c = 0; c < 4; c++) {
+                const int j = c / FL;
+                uint4 b[NT][PIECES];
 #pragma unroll
                 for (int n = 0; n < NT; n++)
 #pragma unroll
-                    for (int p = PIECES - 1; p >= 0; p--) {
-                        mma16816<T>(d[r][n], f[0], b[n][p].x, b[n][p].y, c % FL == 0 && p == PIECES - 1);
-                        mma16816<T>(d[r][n], f[1], b[n][p].z, b[n][p].w, false);
-                    }
-                if (c % FL == FL - 1)
+                    for (int p = 0; p < PIECES; p++) b[n][p] = load_x(xstage, kt, c, n, p);
+#pragma unroll
+                for (int r = 0; r < RB; r++) {
+                    uint32_t f[2][4];
+#pragma unroll
+                    for (int h = 0; h < 2; h++)
+#pragma unroll
+                        for (int k = 0; k < 4; k++) f[h][k] = int_pair<T>(w[r][k & 1][c], 2 * h + k / 2, zz[r][k & 1][j], bits);
 #pragma unroll
                     for (int n = 0; n < NT; n++)
 #pragma unroll
-                        for (int k = 0; k < 4; k++) acc[r][n][k] = fmaf(sc[r][k / 2][j], d[r][n][k], acc[r][n][k]);
+                        for (int p = PIECES - 1; p >= 0; p--) {
+                            mma16816<T>(d[r][n], f[0], b[n][p].x, b[n][p].y, c % FL == 0 && p == PIECES - 1);
+                            mma16816<T>(d[r][n], f[1], b[n][p].z, b[n][p].w, false);
+                        }
+                    if (c % FL == FL - 1)
+#pragma unroll
+                        for (int n = 0; n < NT; n++)
+#pragma unroll
+                            for (int k = 0; k < 4; k++) acc[r][n][k] = fmaf(sc[r][k / 2][j], d[r][n][k], acc[r][n][k]);
+                }
             }
         }
     }
@@ -425,14 +441,19 @@ int grid_n(const llmc_ctx* ctx, int64_t items) {
 template <typename T, typename O, int NT, int PIECES, int NG, int RB>
 llmc_status launch_few(llmc_ctx* ctx, const FewArgs& a, cudaStream_t st) {
     constexpr auto kernel = few_kernel<T, O, NT, PIECES, NG, RB>;
-    constexpr int REC = 1024 + 80 * NG, STAGES = few_stages(RB);
+    constexpr int REC = 1024 + 80 * NG, STAGES = few_stages(NT, RB), FEW_TILES = few_tiles(NT, RB);
+    static std::atomic<bool> ready[64];
     const int64_t blocks = (a.v.rows + ROWS * RB - 1) / (ROWS * RB);
     const int ktiles = (int)(a.v.kp / TILE), tiles = (a.tokens + 8 * NT - 1) / (8 * NT);
-    const int warps = ktiles < FEW_WARPS ? ktiles : FEW_WARPS, toks = a.tokens < 8 * NT ? a.tokens : 8 * NT;
-    size_t sm = 16 + (size_t)warps * STAGES * (RB * REC + (PIECES == 1 ? toks * 256 : 0)), sums = (size_t)warps * 8 * NT * ROWS * RB * sizeof(float);
+    const int steps = (ktiles + FEW_TILES - 1) / FEW_TILES, warps = steps < FEW_WARPS ? steps : FEW_WARPS, toks = a.tokens < 8 * NT ? a.tokens : 8 * NT;
+    size_t sm = 16 + (size_t)warps * STAGES * FEW_TILES * (RB * REC + (PIECES == 1 ? toks * 256 : 0)), sums = (size_t)warps * 8 * NT * ROWS * RB * sizeof(float);
     if (sm < sums) sm = sums;
-    static_assert(16 + FEW_WARPS * STAGES * (RB * REC + (PIECES == 1 ? 8 * NT * 256 : 0)) <= 227 * 1024, "shared memory of an SM");
-    LLMC_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sm));
+    constexpr int MOST = 16 + FEW_WARPS * STAGES * FEW_TILES * (RB * REC + (PIECES == 1 ? 8 * NT * 256 : 0));
+    static_assert(MOST <= 227 * 1024, "shared memory of an SM");
+    if (ctx->device < 0 || ctx->device >= 64 || !ready[ctx->device].load(std::memory_order_relaxed)) {
+        LLMC_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, MOST));
+        if (ctx->device >= 0 && ctx->device < 64) ready[ctx->device].store(true, std::memory_order_relaxed);
+    }
     kernel<<<dim3((unsigned)blocks, (unsigned)tiles), warps * 32, sm, st>>>(a);
     return check_launch(ctx, "int4_few");
 }

@@ -209,6 +209,19 @@ def test_products_and_gradients(tokens, m, n, dtype, strategy, group, sym):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_products_of_few_tokens_on_the_tensor_cores(dtype):
+    """A weight large enough that 40 tokens leave the few-row kernel, rows and columns off the tiles."""
+    from llmcompressorsharp_b200 import int4_linear
+
+    e, w = entry(4201, 4103, group=64, pow2=True, device=ROOT_DEV)
+    x = torch.randint(-4, 5, (40, 4103), generator=torch.Generator().manual_seed(0)).double()
+    b = torch.randint(-4, 5, (4201,), generator=torch.Generator().manual_seed(1)).double()
+    y = int4_linear(x.to(ROOT_DEV, dtype), weight(e, 4103), b.to(ROOT_DEV, dtype))
+    assert torch.equal(y.cpu(), (x @ w.t() + b).float().to(dtype))
+
+
+@pytest.mark.gpu
 def test_gradient_against_differences():
     """The product is linear in x: a step of t along d changes it by t (d W^T), whatever x is."""
     from llmcompressorsharp_b200 import int4_linear
