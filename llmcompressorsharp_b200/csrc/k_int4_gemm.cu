@@ -43,8 +43,8 @@ using namespace w4;
 
 constexpr int BOX = 64;                       // columns of a TMA box: 128 bytes, the swizzle's width
 constexpr int BOX_BYTES = 128 * BOX * 2;
-constexpr int STAGES = 3, A_BYTES = 2 * BOX_BYTES, B_BYTES = 2 * BOX_BYTES, STAGE_BYTES = A_BYTES + B_BYTES;
-constexpr int CODE_STAGES = 3, CODE_BYTES = (TILE / ROWS) * (1024 + 80 * MAX_NG);  // tiles of codes
+constexpr int STAGES = 2, A_BYTES = 2 * BOX_BYTES, B_BYTES = 2 * BOX_BYTES, STAGE_BYTES = A_BYTES + B_BYTES;
+constexpr int CODE_STAGES = 4, CODE_BYTES = (TILE / ROWS) * (1024 + 80 * MAX_NG);  // tiles of codes
 constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + CODE_STAGES * CODE_BYTES + 1024 + 256;
 static_assert(SMEM_BYTES <= 227 * 1024, "shared memory of a CTA");
 constexpr int DQ_WARPS = 8;
@@ -138,13 +138,9 @@ __device__ __forceinline__ uint4 dequant(uint32_t word, const Scale<T, PIECES>& 
     return make_uint4(o[0], o[1], o[2], o[3]);
 }
 
-template <int CG> __device__ __forceinline__ void commit(uint64_t* bar) {
-    if constexpr (CG == 2) umma2_commit_mc(bar, 0x3);
-    else umma_commit(bar);
-}
-
-// T: operand type; O: output (and bias) type; DIR 0 forward, 1 gradient; CG CTAs per tile; PIECES 1, or 3 for fp32.
-template <typename T, typename O, int DIR, int CG, int PIECES>
+// T: operand type; O: output (and bias) type; DIR 0 forward, 1 gradient; CG CTAs per tile; PIECES 1, or 3 for fp32; ONE
+// group to a tile's columns (whose scales a thread then keeps once), or up to four.
+template <typename T, typename O, int DIR, int CG, int PIECES, bool ONE>
 __global__ void __launch_bounds__(32 * (3 + (PIECES == 3 ? 8 : 4) + DQ_WARPS), 1)
     gemm_int4_kernel(const __grid_constant__ CUtensorMap amap, const __grid_constant__ GemmInt4 a) {
     constexpr bool FOLDS = PIECES == 3;
@@ -255,38 +251,42 @@ __global__ void __launch_bounds__(32 * (3 + (PIECES == 3 ? 8 : 4) + DQ_WARPS), 1
         }
         __syncwarp();
     } else if (warp == 1) {
-        if (lane == 0 && rank == 0) {
-            // ---- MMA
-            for (int un = worker; un < units && !*abort_flag; un += workers) {
+        if (rank == 0) {
+            // ---- MMA, issued by one lane of the converged warp; what is computed between two is time between two, so the
+            // descriptors are built once: a stage's and a step's differ from them in the address's low word only.
+            const uint32_t base = smem_u32(smem);
+            const uint64_t desc_a = smem_desc_k_sw128(base);
+            const uint64_t desc_b = DIR == 0 ? smem_desc_k_sw128(base + A_BYTES) : smem_desc_mn_sw128(base + A_BYTES, BOX_BYTES);
+            const auto desc_at = [](uint64_t d, uint32_t off) { return (d & 0xFFFFFFFF00000000ull) | ((uint32_t)d + off); };
+            const auto ready = [&](uint64_t* bar, uint32_t parity) {
+                return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, a.err, a.wait_limit)) != 0;
+            };
+            for (int un = worker; un < units; un += workers) {
                 const Unit u = unit_at<CG>(a, un);
                 bool open = false;
                 const bool ok = tiles(u, [&](int, int, int, bool first, bool last) {
                     const int b = (int)(cc & 1u);
                     if (first) {
-                        if (!mbar_wait(&tempty[b], ((cc >> 1) & 1u) ^ 1u, abort_flag, a.err, a.wait_limit)) return false;
+                        if (!ready(&tempty[b], ((cc >> 1) & 1u) ^ 1u)) return false;
                         tc_fence_after();
                         open = true;
                     }
                     const int s = it % STAGES;
                     const uint32_t ph = (it / STAGES) & 1u;
-                    if (!mbar_wait(&afull[s], ph, abort_flag, a.err, a.wait_limit)) return false;
-                    if (!mbar_wait(&bfull[s], ph, abort_flag, a.err, a.wait_limit)) return false;
+                    if (!ready(&afull[s], ph) || !ready(&bfull[s], ph)) return false;
                     tc_fence_after();
-                    const uint32_t abase = smem_u32(smem + s * STAGE_BYTES), bbase = abase + A_BYTES;
                     const uint32_t dst = tmem + (uint32_t)(b * BN);
+                    const uint32_t at = (uint32_t)(s * (STAGE_BYTES >> 4));
 #pragma unroll
                     for (int kk = 0; kk < TILE / 16; kk++) {
-                        const uint32_t k = kk / 4 * BOX_BYTES + kk % 4 * 32;  // K-major: 16 columns are 32 bytes of a box
-                        const uint64_t da = smem_desc_k_sw128(abase + k);
-                        const uint64_t db = DIR == 0 ? smem_desc_k_sw128(bbase + k) : smem_desc_mn_sw128(bbase + kk * 2048, BOX_BYTES);
-                        const uint32_t acc = first && kk == 0 ? 0u : 1u;
-                        if constexpr (CG == 2) umma2_f16(dst, da, db, a.idesc, acc);
-                        else umma_f16(dst, da, db, a.idesc, acc);
+                        const uint32_t k = (kk / 4 * BOX_BYTES + kk % 4 * 32) >> 4;  // K-major: 16 columns are 32 bytes of a box
+                        const uint64_t da = desc_at(desc_a, at + k), db = desc_at(desc_b, at + (DIR == 0 ? k : kk * (2048 >> 4)));
+                        umma_f16_warp<CG>(dst, da, db, a.idesc, first && kk == 0 ? 0u : 1u);
                     }
-                    commit<CG>(&empty[s]);
+                    umma_commit_warp<CG>(&empty[s]);
                     it++;
                     if (last) {
-                        commit<CG>(&tfull[b]);
+                        umma_commit_warp<CG>(&tfull[b]);
                         commit_par[b] = (int)((cc >> 1) & 1u);
                         open = false;
                         cc++;
@@ -295,7 +295,7 @@ __global__ void __launch_bounds__(32 * (3 + (PIECES == 3 ? 8 : 4) + DQ_WARPS), 1
                 });
                 if (!ok) {
                     if (open) {  // so that the tail can wait for what was issued
-                        commit<CG>(&tfull[cc & 1u]);
+                        umma_commit_warp<CG>(&tfull[cc & 1u]);
                         commit_par[cc & 1u] = (int)((cc >> 1) & 1u);
                     }
                     break;
@@ -417,8 +417,9 @@ __global__ void __launch_bounds__(32 * (3 + (PIECES == 3 ? 8 : 4) + DQ_WARPS), 1
         }
     } else if (warp < 2 + EW + DQ_WARPS) {
         // ---- dequantising
-        const int grp = (warp - 2 - EW) / 4, w = (warp - 2 - EW) % 4, ng = a.v.ng, t = lane & 3, r8 = row_of(lane);
+        const int grp = (warp - 2 - EW) / 4, w = (warp - 2 - EW) % 4, ng = ONE ? 1 : a.v.ng, t = lane & 3, r8 = row_of(lane);
         const int64_t lim = (DIR == 0 ? a.v.mp : a.v.kp) - 128;
+        constexpr int GROUPS = ONE ? 1 : 4;
         const Bits bits = get_bits(slot);
         for (int un = worker; un < units && !*abort_flag; un += workers) {
             const Unit u = unit_at<CG>(a, un);
@@ -446,7 +447,7 @@ __global__ void __launch_bounds__(32 * (3 + (PIECES == 3 ? 8 : 4) + DQ_WARPS), 1
                 }
                 const unsigned char* tile = codes + cs * CODE_BYTES;
                 uint4 q[4];
-                Scale<T, PIECES> sc[4][4];
+                Scale<T, PIECES> sc[4][GROUPS];
 #pragma unroll
                 for (int i = 0; i < 4; i++) {
                     const unsigned char* rec = tile + (2 * w + i / 2) * a.v.rec;
@@ -455,13 +456,8 @@ __global__ void __launch_bounds__(32 * (3 + (PIECES == 3 ? 8 : 4) + DQ_WARPS), 1
                     const float* scales = reinterpret_cast<const float*>(rec + 1024) + in * ng;
                     const unsigned char* zeros = rec + 1024 + 64 * ng + in * ng;
 #pragma unroll
-                    for (int c = 0; c < 4; c++) {
-                        if (c && ng == 1) {
-                            sc[i][c] = sc[i][0];
-                            continue;
-                        }
+                    for (int c = 0; c < GROUPS; c++)
                         sc[i][c].set(scales[slot_of(c, ng)] * e[DIR == 0 ? i : c], zeros[slot_of(c, ng)]);
-                    }
                 }
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&cempty[cs]);
@@ -474,7 +470,7 @@ __global__ void __launch_bounds__(32 * (3 + (PIECES == 3 ? 8 : 4) + DQ_WARPS), 1
                     for (int c = 0; c < 4; c++) {
                         // K-major and MN-major alike: a box holds 64 layout columns of 128 rows, rows of 128 bytes
                         const int off = c / 2 * BOX_BYTES + (32 * w + 8 * i + r8) * 128 + (((4 * (c & 1) + t) ^ r8) << 4);
-                        *reinterpret_cast<uint4*>(b + off) = dequant<T, PIECES>(word[c], sc[i][c], bits, wp);
+                        *reinterpret_cast<uint4*>(b + off) = dequant<T, PIECES>(word[c], sc[i][ONE ? 0 : c], bits, wp);
                     }
                 }
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -586,9 +582,9 @@ template <auto kernel> int max_workers(llmc_ctx* ctx, int cg, int threads) {
     return cache[dev];
 }
 
-template <typename T, typename O, int DIR, int CG, int PIECES>
-llmc_status launch(llmc_ctx* ctx, cudaStream_t st, const CUtensorMap& map, GemmInt4& g) {
-    constexpr auto kernel = gemm_int4_kernel<T, O, DIR, CG, PIECES>;
+template <typename T, typename O, int DIR, int CG, int PIECES, bool ONE>
+llmc_status launch_as(llmc_ctx* ctx, cudaStream_t st, const CUtensorMap& map, GemmInt4& g) {
+    constexpr auto kernel = gemm_int4_kernel<T, O, DIR, CG, PIECES, ONE>;
     constexpr int threads = 32 * (3 + (PIECES == 3 ? 8 : 4) + DQ_WARPS);
     int cap = max_workers<kernel>(ctx, CG, threads);
     const int allowed = persistent_sms(ctx) / CG;
@@ -609,6 +605,11 @@ llmc_status launch(llmc_ctx* ctx, cudaStream_t st, const CUtensorMap& map, GemmI
     cfg.numAttrs = 1;
     LLMC_CUDA_TRY(cudaLaunchKernelEx(&cfg, kernel, map, g));
     return check_launch(ctx, "int4_gemm");
+}
+
+template <typename T, typename O, int DIR, int CG, int PIECES>
+llmc_status launch(llmc_ctx* ctx, cudaStream_t st, const CUtensorMap& map, GemmInt4& g) {
+    return g.v.ng == 1 ? launch_as<T, O, DIR, CG, PIECES, true>(ctx, st, map, g) : launch_as<T, O, DIR, CG, PIECES, false>(ctx, st, map, g);
 }
 
 }  // namespace

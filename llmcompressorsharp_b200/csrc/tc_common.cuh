@@ -101,6 +101,43 @@ __device__ __forceinline__ void umma_f16(uint32_t tmem_d, uint64_t da, uint64_t 
         : "memory");
 }
 
+// The same issued by one lane of a converged warp: the operands stay in uniform registers, where an MMA of a branch for
+// one lane fetches each of them from that lane's first.  elect.sync names the same lane every time.
+template <int CG> __device__ __forceinline__ void umma_f16_warp(uint32_t tmem_d, uint64_t da, uint64_t db, uint32_t idesc, uint32_t acc) {
+    if constexpr (CG == 2)
+        asm volatile(
+            "{\n\t.reg .pred p, q;\n\t"
+            "setp.ne.b32 p, %4, 0;\n\t"
+            "elect.sync _|q, 0xffffffff;\n\t"
+            "@q tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, {%5, %5, %5, %5, %5, %5, %5, %5}, p;\n\t}"
+            ::"r"(tmem_d), "l"(da), "l"(db), "r"(idesc), "r"(acc), "r"(0u)
+            : "memory");
+    else
+        asm volatile(
+            "{\n\t.reg .pred p, q;\n\t"
+            "setp.ne.b32 p, %4, 0;\n\t"
+            "elect.sync _|q, 0xffffffff;\n\t"
+            "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, {%5, %5, %5, %5}, p;\n\t}"
+            ::"r"(tmem_d), "l"(da), "l"(db), "r"(idesc), "r"(acc), "r"(0u)
+            : "memory");
+}
+// The commit of those MMAs, to a pair's both CTAs (CG = 2).
+template <int CG> __device__ __forceinline__ void umma_commit_warp(uint64_t* bar) {
+    if constexpr (CG == 2)
+        asm volatile(
+            "{\n\t.reg .pred q;\n\t"
+            "elect.sync _|q, 0xffffffff;\n\t"
+            "@q tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;\n\t}" ::"r"(smem_u32(bar)),
+            "h"((uint16_t)3)
+            : "memory");
+    else
+        asm volatile(
+            "{\n\t.reg .pred q;\n\t"
+            "elect.sync _|q, 0xffffffff;\n\t"
+            "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(smem_u32(bar))
+            : "memory");
+}
+
 __device__ __forceinline__ void umma_commit(uint64_t* bar) {
     asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar))
                  : "memory");
