@@ -414,22 +414,25 @@ __global__ void __launch_bounds__(256) join_kernel(const float* part, int splits
     }
 }
 
-// part[split][c] = sum of rows split * per .. of x[:, c]; a block holds 32 columns x 8 row lanes.
+// part[split][c] = sum of rows split * per .. of x[:, c], or (one split) out[c] rounded; a block holds 32 columns x
+// 8 row lanes.
 template <typename T>
-__global__ void __launch_bounds__(256) colsum_kernel(const T* x, int64_t rows, int64_t cols, int64_t ld, int64_t per, float* part) {
+__global__ void __launch_bounds__(256) colsum_kernel(const T* x, int64_t rows, int64_t cols, int64_t ld, int64_t per, float* part, T* out) {
     __shared__ float sm[8][33];
     const int lane = threadIdx.x % 32, w = threadIdx.x / 32;
     const int64_t c = (int64_t)blockIdx.x * 32 + lane;
     const int64_t r0 = blockIdx.y * per, r1 = min(rows, r0 + per);
     float s = 0.f;
     if (c < cols)
+#pragma unroll 4
         for (int64_t r = r0 + w; r < r1; r += 8) s += to_f<T>(x[r * ld + c]);
     sm[w][lane] = s;
     __syncthreads();
     if (w == 0 && c < cols) {
 #pragma unroll
         for (int i = 1; i < 8; i++) s += sm[i][lane];
-        part[blockIdx.y * cols + c] = s;
+        if (out) out[c] = from_f<T>(s);
+        else part[blockIdx.y * cols + c] = s;
     }
 }
 
@@ -540,14 +543,17 @@ llmc_status int4_join(llmc_ctx* ctx, cudaStream_t st, const float* part, int spl
     return check_launch(ctx, "int4_join");
 }
 
-llmc_status col_sum_parts(llmc_ctx* ctx, cudaStream_t st, const void* x, int dtype, int64_t rows, int64_t cols, int64_t ld,
-                          int splits, float* part) {
+llmc_status col_sum(llmc_ctx* ctx, cudaStream_t st, const void* x, int dtype, int64_t rows, int64_t cols, int64_t ld, int splits,
+                    float* part, void* out) {
     const dim3 grid((unsigned)((cols + 31) / 32), (unsigned)splits);
     const int64_t per = (rows + splits - 1) / splits;
-    if (dtype == LLMC_DTYPE_F32) colsum_kernel<float><<<grid, 256, 0, st>>>((const float*)x, rows, cols, ld, per, part);
-    else if (dtype == LLMC_DTYPE_BF16) colsum_kernel<__nv_bfloat16><<<grid, 256, 0, st>>>((const __nv_bfloat16*)x, rows, cols, ld, per, part);
-    else colsum_kernel<__half><<<grid, 256, 0, st>>>((const __half*)x, rows, cols, ld, per, part);
-    return check_launch(ctx, "col_sum");
+    void* direct = splits == 1 ? out : nullptr;
+    if (dtype == LLMC_DTYPE_F32) colsum_kernel<float><<<grid, 256, 0, st>>>((const float*)x, rows, cols, ld, per, part, (float*)direct);
+    else if (dtype == LLMC_DTYPE_BF16)
+        colsum_kernel<__nv_bfloat16><<<grid, 256, 0, st>>>((const __nv_bfloat16*)x, rows, cols, ld, per, part, (__nv_bfloat16*)direct);
+    else colsum_kernel<__half><<<grid, 256, 0, st>>>((const __half*)x, rows, cols, ld, per, part, (__half*)direct);
+    LLMC_TRY(check_launch(ctx, "col_sum"));
+    return splits == 1 ? LLMC_OK : int4_join(ctx, st, part, splits, 1, cols, nullptr, out, dtype, cols);
 }
 
 }  // namespace llmc

@@ -83,11 +83,12 @@ llmc_status int4_few(llmc_ctx* ctx, cudaStream_t st, const w4::View& v, const vo
 int int4_gemm_splits(const llmc_ctx* ctx, int dtype, int64_t tokens, int64_t cols, int64_t contraction);
 llmc_status int4_gemm(llmc_ctx* ctx, cudaStream_t st, const w4::View& v, int dir, int dtype, const void* A, int64_t acols,
                       int64_t lda, int64_t tokens, const void* bias, void* out, int64_t ldo, int splits, float* part);
-// out = sum of `splits` fp32 parts in order, + bias; and the column sums of x as parts.
+// out = sum of `splits` fp32 parts in order, + bias.
 llmc_status int4_join(llmc_ctx* ctx, cudaStream_t st, const float* part, int splits, int64_t rows, int64_t cols, const void* bias,
                       void* out, int dtype, int64_t ldo);
-llmc_status col_sum_parts(llmc_ctx* ctx, cudaStream_t st, const void* x, int dtype, int64_t rows, int64_t cols, int64_t ld,
-                          int splits, float* part);
+// out = column sums of x, the rows in `splits` parts.
+llmc_status col_sum(llmc_ctx* ctx, cudaStream_t st, const void* x, int dtype, int64_t rows, int64_t cols, int64_t ld, int splits,
+                    float* part, void* out);
 
 // ---- embedding (k_embedding.cu) ----------------------------------------------------------------
 llmc_status embedding_lookup(llmc_ctx* ctx, cudaStream_t st, const void* ids, int ids64, int64_t tokens, const void* table, int dtype,

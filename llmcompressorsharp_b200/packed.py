@@ -141,31 +141,38 @@ class Int4Weight:
                   self.shape[1])
         return out
 
-    def _workspace(self, fn: str, a: torch.Tensor, code: int, tokens: int, ld: int):
-        """Scratch tensor (or None) of one product; its size depends on what the key holds."""
-        key = (fn, code, tokens, ld, a.data_ptr() % 16)
+    def _workspace(self, fn: str, at: int, code: int, tokens: int, ld: int):
+        """Scratch tensor (or None) of one product of the rows at address ``at``; its size depends on what the key holds."""
+        key = (fn, code, tokens, ld, at % 16)
         need = self._need.get(key)
         if need is None:
             v = _lib.I64()
-            _lib.call(fn, self._ctx, self._ref, a.data_ptr(), code, tokens, ld, C.byref(v))
+            _lib.call(fn, self._ctx, self._ref, at, code, tokens, ld, C.byref(v))
             if len(self._need) >= 256:
                 self._need.clear()
             need = self._need[key] = v.value
         return torch.empty(need, dtype=torch.uint8, device=self.device) if need else None
 
-    def _product(self, x2: torch.Tensor, bias, back: bool) -> torch.Tensor:
-        code, tokens, ld = _DTYPES[x2.dtype], x2.shape[0], _pitch(x2)
-        out = torch.empty(tokens, self.shape[1 if back else 0], dtype=x2.dtype, device=self.device)
+    def _product(self, x: torch.Tensor, bias, back: bool) -> torch.Tensor:
+        """x [..., cols] W^T + bias, or (back) x [..., rows] W; a new tensor [..., rows] or [..., cols]."""
+        last = self.shape[0 if back else 1]
+        if x.is_contiguous():
+            a, tokens, ld = x, x.numel() // last, last
+        else:
+            a = _rows(x, last)
+            tokens, ld = a.shape[0], _pitch(a)
+        n = self.shape[1 if back else 0]
+        out = x.new_empty(*x.shape[:-1], n)
         if tokens == 0:
             return out
-        ws = self._workspace("llmc_int4_linear_grad_workspace" if back else "llmc_int4_linear_workspace", x2, code, tokens, ld)
+        code, at = _DTYPES[a.dtype], a.data_ptr()
+        ws = self._workspace("llmc_int4_linear_grad_workspace" if back else "llmc_int4_linear_workspace", at, code, tokens, ld)
         wp, wn = (ws.data_ptr(), ws.numel()) if ws is not None else (None, 0)
         if back:
-            _lib.call("llmc_int4_linear_grad", self._ctx, _lib.stream(self._index), self._ref, x2.data_ptr(), code, tokens, ld,
-                      out.data_ptr(), out.shape[1], wp, wn)
+            _lib.call("llmc_int4_linear_grad", self._ctx, _lib.stream(self._index), self._ref, at, code, tokens, ld, out.data_ptr(), n, wp, wn)
         else:
-            _lib.call("llmc_int4_linear", self._ctx, _lib.stream(self._index), self._ref, x2.data_ptr(), code, tokens, ld,
-                      bias.data_ptr() if bias is not None else None, out.data_ptr(), out.shape[1], wp, wn)
+            _lib.call("llmc_int4_linear", self._ctx, _lib.stream(self._index), self._ref, at, code, tokens, ld,
+                      bias.data_ptr() if bias is not None else None, out.data_ptr(), n, wp, wn)
         return out
 
 
@@ -199,16 +206,15 @@ def _col_sum(x2: torch.Tensor) -> torch.Tensor:
 class _Int4LinearFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx_, x, weight, bias):
-        ctx_.weight, ctx_.shape = weight, x.shape
-        return weight._product(_rows(x, weight.shape[1]), bias, False).reshape(*x.shape[:-1], weight.shape[0])
+        ctx_.weight = weight
+        return weight._product(x, bias, False)
 
     @staticmethod
     @once_differentiable
     def backward(ctx_, dy):
         w = ctx_.weight
-        d2 = _rows(dy, w.shape[0])
-        dx = w._product(d2, None, True).reshape(ctx_.shape) if ctx_.needs_input_grad[0] else None
-        db = _col_sum(d2) if ctx_.needs_input_grad[2] else None
+        dx = w._product(dy, None, True) if ctx_.needs_input_grad[0] else None
+        db = _col_sum(_rows(dy, w.shape[0])) if ctx_.needs_input_grad[2] else None
         return dx, None, db
 
 
@@ -237,12 +243,11 @@ def int4_linear(x: torch.Tensor, weight: Int4Weight, bias: torch.Tensor | None =
             bias = bias.contiguous()
     if torch.is_grad_enabled() and (x.requires_grad or (bias is not None and bias.requires_grad)):
         return _Int4LinearFn.apply(x, weight, bias)
-    y = weight._product(_rows(x, cols), bias, False)
-    return y if x.dim() == 2 else y.reshape(*x.shape[:-1], rows)
+    return weight._product(x, bias, False)
 
 
 def _lookup(ids, table, scale):
-    out = torch.empty(ids.numel(), table.shape[1], dtype=table.dtype, device=table.device)
+    out = table.new_empty(*ids.shape, table.shape[1])
     index = table.device.index
     _lib.call("llmc_embedding", _lib.ctx_handle(index), _lib.stream(index), ids.data_ptr(), int(ids.dtype == torch.int64),
               ids.numel(), table.data_ptr(), _DTYPES[table.dtype], table.shape[0], table.shape[1], _pitch(table), scale,
@@ -255,7 +260,7 @@ class _EmbeddingFn(torch.autograd.Function):
     def forward(ctx_, table, ids, scale, padding):
         ctx_.save_for_backward(ids)
         ctx_.scale, ctx_.padding, ctx_.shape = scale, padding, table.shape
-        return _lookup(ids.reshape(-1), table, scale).reshape(*ids.shape, table.shape[1])
+        return _lookup(ids, table, scale)
 
     @staticmethod
     @once_differentiable
@@ -319,7 +324,7 @@ def embedding(ids: torch.Tensor, table, scale: float = 1.0, padding_idx: int | N
     table = _rows(table, hidden)
     if torch.is_grad_enabled() and table.requires_grad:
         return _EmbeddingFn.apply(table, ids, scale, padding)
-    return _lookup(ids.reshape(-1), table, scale).reshape(*ids.shape, hidden)
+    return _lookup(ids, table, scale)
 
 
 class Int4Linear(torch.nn.Module):

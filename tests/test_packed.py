@@ -256,14 +256,14 @@ def test_strides_alignment_and_surroundings(tokens):
         assert torch.equal(int4_linear(x.reshape(1, tokens, n), p).cpu(), want[None])
     x = big[:, :n].contiguous()
     y = torch.full((tokens + 2, m + 5), 7.0, dtype=torch.bfloat16, device=ROOT_DEV)
-    ws = p._workspace("llmc_int4_linear_workspace", x, _lib.DTYPE_BF16, tokens, n)
+    ws = p._workspace("llmc_int4_linear_workspace", x.data_ptr(), _lib.DTYPE_BF16, tokens, n)
     _lib.call("llmc_int4_linear", p._ctx, _lib.stream(0), p._ref, x.data_ptr(), _lib.DTYPE_BF16, tokens, n, None, y.data_ptr(), m + 5,
               ws.data_ptr() if ws is not None else None, ws.numel() if ws is not None else 0)
     assert torch.equal(y[:tokens, :m].cpu(), (x.double().cpu() @ w.t()).float().to(torch.bfloat16))
     assert bool((y[tokens:] == 7).all()) and bool((y[:, m:] == 7).all())
     d = torch.full((tokens + 2, n + 3), 7.0, dtype=torch.bfloat16, device=ROOT_DEV)
     dy = y[:tokens, :m].contiguous()
-    ws = p._workspace("llmc_int4_linear_grad_workspace", dy, _lib.DTYPE_BF16, tokens, m)
+    ws = p._workspace("llmc_int4_linear_grad_workspace", dy.data_ptr(), _lib.DTYPE_BF16, tokens, m)
     _lib.call("llmc_int4_linear_grad", p._ctx, _lib.stream(0), p._ref, dy.data_ptr(), _lib.DTYPE_BF16, tokens, m, d.data_ptr(), n + 3,
               ws.data_ptr() if ws is not None else None, ws.numel() if ws is not None else 0)
     assert bool((d[tokens:] == 7).all()) and bool((d[:, n:] == 7).all())
