@@ -88,7 +88,7 @@ __global__ void __launch_bounds__(256) lookup_kernel(const T* table, int64_t ldt
 
 // ---- sorting the tokens -----------------------------------------------------------------------------
 constexpr int SORT_WARPS = 32, SORT_NT = SORT_WARPS * 32;
-constexpr int DIGIT = 9, BINS = 1 << DIGIT, BATCH = 8;
+constexpr int DIGIT = 9, BINS = 1 << DIGIT, BATCH = 8, MAX_CTAS = 16;
 // Tokens that one row sums by itself; a longer run is cut into pieces of this many.  A piece costs a
 // partial row in fp32 (an eighth of what its 32 bf16 rows cost to read, written and read again), a long
 // run costs its serial sum.
@@ -128,7 +128,7 @@ __global__ void __launch_bounds__(SORT_NT) sort_kernel(const I* ids, uint32_t to
     if (rank == 0 && threadIdx.x < 2) p.counts[threadIdx.x] = 0;
 
     // Each warp takes its stretch in batches of BATCH x 32 tokens, whose keys it loads at once: one latency a batch
-    // instead of one for each 32 tokens (60 us became 20 for 65,536 of them).
+    // instead of one for each 32 tokens.  65,536 tokens take 22 us (60 with single loads, a cluster of eight and matches).
     uint2 pair[BATCH];  // token, id
     bool bad = false;
     auto load = [&](int pass, uint32_t i0) {
@@ -156,35 +156,40 @@ __global__ void __launch_bounds__(SORT_NT) sort_kernel(const I* ids, uint32_t to
             load(pass, i);
 #pragma unroll
             for (int q = 0; q < BATCH; q++) {
-                const bool in = i + q * 32 + lane < last;
-                const unsigned live = __ballot_sync(0xffffffffu, in);
-                if (in) {
-                    const uint32_t d = (pair[q].y >> shift) & (bins - 1);
-                    const unsigned peers = __match_any_sync(live, d);
-                    if ((peers & ((1u << lane) - 1)) == 0) mine[d] += __popc(peers);
-                }
-                __syncwarp();
+                if (i + q * 32 + lane < last) atomicAdd(&mine[(pair[q].y >> shift) & (bins - 1)], 1u);
             }
         }
         __syncthreads();
         if ((int)threadIdx.x < bins) {  // exclusive over the warps
             uint32_t s = 0;
-            for (int w = 0; w < SORT_WARPS; w++) {
-                const uint32_t c = hist[w * BINS + threadIdx.x];
-                hist[w * BINS + threadIdx.x] = s;
-                s += c;
+#pragma unroll
+            for (int w0 = 0; w0 < SORT_WARPS; w0 += 8) {
+                uint32_t c[8];
+#pragma unroll
+                for (int w = 0; w < 8; w++) c[w] = hist[(w0 + w) * BINS + threadIdx.x];
+#pragma unroll
+                for (int w = 0; w < 8; w++) {
+                    hist[(w0 + w) * BINS + threadIdx.x] = s;
+                    s += c[w];
+                }
             }
             total[threadIdx.x] = s;
         }
         cluster_sync();
         uint32_t before = 0, all = 0;
-        if ((int)threadIdx.x < bins)
-            for (uint32_t c = 0; c < ctas; c++) {
-                uint32_t n;
-                asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(n) : "r"(mapa_shared(tc::smem_u32(&total[threadIdx.x]), c)));
-                if (c < rank) before += n;
-                all += n;
+        if ((int)threadIdx.x < bins) {
+            uint32_t n[MAX_CTAS];  // all under way before the first is used
+#pragma unroll
+            for (uint32_t c = 0; c < MAX_CTAS; c++) {
+                n[c] = 0;
+                if (c < ctas) asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(n[c]) : "r"(mapa_shared(tc::smem_u32(&total[threadIdx.x]), c)));
             }
+#pragma unroll
+            for (uint32_t c = 0; c < MAX_CTAS; c++) {
+                if (c < rank) before += n[c];
+                all += n[c];
+            }
+        }
         uint32_t inc = all;  // inclusive over the bins, by warp and then over the warps
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -203,13 +208,16 @@ __global__ void __launch_bounds__(SORT_NT) sort_kernel(const I* ids, uint32_t to
             if (last - first > 32 * BATCH) load(pass, i);  // else the batch counted is the one to place
 #pragma unroll
             for (int q = 0; q < BATCH; q++) {
+                if (i + q * 32 >= last) break;
+                // the lanes of the same digit, a vote to a bit (a match instruction took 40 clocks of the SM each)
                 const bool in = i + q * 32 + lane < last;
-                const unsigned live = __ballot_sync(0xffffffffu, in);
-                unsigned peers = 0;
-                uint32_t d = 0;
+                const uint32_t d = (pair[q].y >> shift) & (bins - 1);
+                unsigned peers = __ballot_sync(0xffffffffu, in);
+                for (int b = 0; b < bits; b++) {
+                    const unsigned ones = __ballot_sync(0xffffffffu, d >> b & 1u);
+                    peers &= d >> b & 1u ? ones : ~ones;
+                }
                 if (in) {
-                    d = (pair[q].y >> shift) & (bins - 1);
-                    peers = __match_any_sync(live, d);
                     const uint32_t pos = base[d] + mine[d] + __popc(peers & ((1u << lane) - 1));
                     __stcg(p.pairs(pass) + pos, pair[q]);
                 }
