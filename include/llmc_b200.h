@@ -381,8 +381,9 @@ llmc_status llmc_int4_layout(llmc_ctx* ctx, void* stream, const uint8_t* codes, 
 llmc_status llmc_int4_dequantize(llmc_ctx* ctx, void* stream, const llmc_int4_weight* w, int32_t dtype, void* out,
                                  int64_t ldo);
 /* y [tokens, ldy] = x [tokens, ldx] W^T + bias (bias [rows], may be NULL), all of dtype.  Sums in fp32,
- * one rounding.  Up to 16 tokens the codes enter as exact integers; above, and in the gradient, W is
- * rounded to a 16-bit dtype first, or kept to 24 bits for F32. */
+ * one rounding.  With few tokens (16 and fewer always, up to 256 for a small weight) the codes enter as
+ * exact integers; with more, and in the gradient, W is rounded to a 16-bit dtype first, or kept to 24
+ * bits for F32.  The sums of integers times x come before the scale: they must stay in fp32's range. */
 llmc_status llmc_int4_linear_workspace(llmc_ctx* ctx, const llmc_int4_weight* w, const void* x, int32_t dtype,
                                        int64_t tokens, int64_t ldx, int64_t* bytes);
 llmc_status llmc_int4_linear(llmc_ctx* ctx, void* stream, const llmc_int4_weight* w, const void* x, int32_t dtype,
@@ -398,7 +399,8 @@ llmc_status llmc_col_sum_workspace(llmc_ctx* ctx, int64_t rows, int64_t cols, in
 llmc_status llmc_col_sum(llmc_ctx* ctx, void* stream, const void* x, int32_t dtype, int64_t rows, int64_t cols,
                          int64_t ld, void* out, void* ws, int64_t ws_bytes);
 /* out [tokens, ldo] = scale * table[ids], rounded once; ids int64 (ids64 = 1) or int32.  An id outside
- * [0, vocab) gives a row of zeros; the next llmc_sync reports it as LLMC_ERR_OUT_OF_RANGE. */
+ * [0, vocab) gives a row of zeros; the first llmc_sync after the call's work reports it as
+ * LLMC_ERR_OUT_OF_RANGE. */
 llmc_status llmc_embedding(llmc_ctx* ctx, void* stream, const void* ids, int32_t ids64, int64_t tokens, const void* table,
                            int32_t dtype, int64_t vocab, int64_t hidden, int64_t ldt, float scale, void* out, int64_t ldo);
 /* The same from a packed table, in dtype. */

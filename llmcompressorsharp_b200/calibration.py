@@ -29,7 +29,7 @@ from dataclasses import dataclass
 import torch
 import torch.nn.functional as F
 
-from .packed import embedding, load_compressed
+from .packed import TokenEmbedding, load_compressed
 
 
 @dataclass(frozen=True)
@@ -131,13 +131,6 @@ def _rope(x, cos, sin):
     half = x.shape[-1] // 2
     x1, x2 = x[..., :half], x[..., half:]
     return (x * cos + torch.cat((-x2, x1), dim=-1) * sin).to(x.dtype)
-
-
-class TokenEmbedding(torch.nn.Embedding):
-    """torch.nn.Embedding whose lookup, on a CUDA device, is the library's (the same values)."""
-
-    def forward(self, ids):
-        return embedding(ids, self.weight) if self.weight.is_cuda else super().forward(ids)
 
 
 class _Body(torch.nn.Module):

@@ -19,8 +19,7 @@
 //   zeros   16 rows x ng bytes
 //
 // So whatever a product needs of a tile is one stretch of 8,832 bytes (ng = 1), which one bulk copy brings in, and
-// nothing comes from a second place with a latency of its own.  (Records that stood along the columns instead, for
-// eight copies to a tile, made the products of many rows a fifth slower: a bulk copy costs its issue.)
+// nothing comes from a second place with a latency of its own.
 #pragma once
 #include "common.cuh"
 

@@ -4,7 +4,7 @@
 //   gradient  dx[t][k] = sum_n dy[t][n] W[n][k]
 //
 // The activations (A, K-major) come by TMA; the weight (B) is dequantised by eight warps straight into the
-// shared memory the MMA reads: K-major for the forward product (rows n, 64 columns k to a stage), MN-major for
+// shared memory the MMA reads: K-major for the forward product (rows n, 128 columns k to a stage), MN-major for
 // the gradient (rows n are the contraction, 128 columns k to a CTA), so one copy of the codes serves both and
 // no 16-bit weight is ever written to memory.
 //
@@ -24,8 +24,13 @@
 // single CTAs (128 x 128).  Per CTA: a TMA warp for the activations and one for the codes (a tile of 128 x 128
 // weights in one bulk copy), an MMA warp, epilogue warps, eight dequantising warps, a ring of
 // STAGES x (32 KB activations + 32 KB weights) and one of CODE_STAGES tiles of codes, two accumulators in TMEM.
-// A stage is a whole tile, 128 of the contraction: the MMA thread's two waits and its commit take about 700 clocks,
-// which a stage of 64 (512 clocks of MMAs) did not cover (0.59 us a stage; see the figures at int4_gemm).
+// A stage is a whole tile, 128 of the contraction: the MMA warp's two waits and its commit take some hundreds of
+// clocks, which the MMAs of 64 (512 clocks) did not cover.
+//
+// 4096 -> 14336, 8,192 tokens, bf16: 731 us, 1.32 PFLOP/s, which is what the power limit leaves a large product of the
+// library's too (0.94 of its sustained rate); 813 with one thread issuing the MMAs inside a branch and building its
+// descriptors each time.  2,048 tokens of 4096 -> 4096: 71 to 84 us, and its gradient the same.  At 17 to 128 tokens
+// the eight warps that dequantise bound it: 29 us for 4096 -> 14336, where the codes alone are read in 5.
 // Every wait is bounded.
 #include "int4.cuh"
 #include "ops.h"
@@ -587,9 +592,9 @@ llmc_status launch_as(llmc_ctx* ctx, cudaStream_t st, const CUtensorMap& map, Ge
     constexpr auto kernel = gemm_int4_kernel<T, O, DIR, CG, PIECES, ONE>;
     constexpr int threads = 32 * (3 + (PIECES == 3 ? 8 : 4) + DQ_WARPS);
     int cap = max_workers<kernel>(ctx, CG, threads);
-    const int allowed = persistent_sms(ctx) / CG;
-    if (cap > allowed) cap = allowed;
     if (cap < 1) return fail(LLMC_ERR_CUDA, "the packed product's kernel does not fit this device");
+    const int allowed = persistent_sms(ctx) >= CG ? persistent_sms(ctx) / CG : 1;  // one pair at least
+    if (cap > allowed) cap = allowed;
     const int64_t units = (int64_t)g.tiles_m * g.tiles_n * g.splits;
     const int workers = units < cap ? (int)units : cap;
     cudaLaunchConfig_t cfg = {};
@@ -622,7 +627,8 @@ int int4_gemm_cg(int dtype, int64_t tokens, int64_t cols) { return dtype != LLMC
 int int4_gemm_splits(const llmc_ctx* ctx, int dtype, int64_t tokens, int64_t cols, int64_t contraction) {
     const int cg = int4_gemm_cg(dtype, tokens, cols);
     const int64_t tile = 128 * cg, tiles = ((tokens + tile - 1) / tile) * ((cols + tile - 1) / tile);
-    const int64_t kt = contraction / TILE, workers = persistent_sms(ctx) / cg;
+    // by the device's SMs, not llmc_set_sm_limit's: a workspace that was asked for stays large enough
+    const int64_t kt = contraction / TILE, workers = ctx->sm_count / cg;
     int64_t s = workers / tiles;
     const int64_t most = dtype == LLMC_DTYPE_F32 ? kt : kt / 2;
     if (s > most) s = most;

@@ -66,13 +66,6 @@ __device__ __forceinline__ void tma_load_2d(void* smem_dst, const CUtensorMap* m
         : "memory");
 }
 
-// Bounded wait without an abort flag: for barriers that one warp shares with its own copies only.
-__device__ __forceinline__ bool mbar_wait_bounded(uint64_t* b, uint32_t parity, uint32_t limit) {
-    for (unsigned i = 0; i < limit; i++)
-        if (mbar_try_wait(b, parity)) return true;
-    return false;
-}
-
 // Untiled bulk copy into this CTA's shared memory: addresses 16-byte aligned, bytes a multiple of 16.
 __device__ __forceinline__ void bulk_load(void* smem_dst, const void* src, uint32_t bytes, uint64_t* bar) {
     asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"

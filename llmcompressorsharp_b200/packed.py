@@ -221,9 +221,10 @@ class _Int4LinearFn(torch.autograd.Function):
 def int4_linear(x: torch.Tensor, weight: Int4Weight, bias: torch.Tensor | None = None) -> torch.Tensor:
     """y = x W^T + bias for x [..., cols] of float32, bfloat16 or float16; y [..., rows] of x's type.
 
-    Sums are fp32 and rounded once.  Up to 16 rows of x the codes are multiplied as exact integers; with
-    more, and in the backward pass, W is rounded to x's 16-bit type first (as a dequantised weight of that
-    type is), or kept to 24 bits for float32.  Differentiable in x and the bias."""
+    Sums are fp32 and rounded once.  With few rows of x (16 and fewer always, up to 256 for a small weight) the
+    codes are multiplied as exact integers; with more, and in the backward pass, W is rounded to x's 16-bit
+    type first (as a dequantised weight of that type is), or kept to 24 bits for float32.  Differentiable once,
+    in x and the bias."""
     if x is None or weight is None:
         raise ArgumentError("x and weight must not be null")
     if not isinstance(weight, Int4Weight):
@@ -360,20 +361,35 @@ class Int4Embedding(torch.nn.Module):
         return embedding(ids, self.packed_weight, self.scale, dtype=self.dtype)
 
 
+class TokenEmbedding(torch.nn.Embedding):
+    """``torch.nn.Embedding`` whose lookup, on a CUDA device, is the library's (the same values).  Types and options
+    that it does not take, and other devices, are torch's."""
+
+    def forward(self, ids):
+        w = self.weight
+        if (w.is_cuda and w.dtype in _DTYPES and ids.dtype in (torch.int64, torch.int32)
+                and self.max_norm is None and not self.scale_grad_by_freq and not self.sparse):
+            return embedding(ids, w, padding_idx=self.padding_idx)
+        return super().forward(ids)
+
+
 def load_compressed(model: torch.nn.Module, compressed: dict) -> list[str]:
     """Puts packed modules into ``model`` for the entries of ``state.compressed`` (weight name ->
-    entry): a Linear or Embedding whose ``<module>.weight`` has 4-bit codes is replaced by an Int4Linear /
-    Int4Embedding that returns the old weight's type.  Entries without codes, of more than 4 bits or of
-    other modules stay dense.  Returns the names of the modules replaced."""
+    entry): a Linear or Embedding whose ``<module>.weight`` has 4-bit codes is replaced, wherever the model holds it,
+    by an Int4Linear / Int4Embedding that returns the old weight's type.  Entries without codes, of more than 4 bits
+    or of other modules stay dense: subclasses too, whose forward may compute more, and an Embedding with max_norm.
+    So does a module that was tied to a replaced one's weight.  Returns the names of the modules replaced."""
     if model is None or compressed is None:
         raise ArgumentError("model and compressed must not be null")
-    modules, done = dict(model.named_modules()), []
+    modules, done = dict(model.named_modules(remove_duplicate=False)), []
     for name, entry in compressed.items():
         if not name.endswith(".weight") or entry.get("codes") is None or entry["num_bits"] > 4:
             continue
         path = name[: -len(".weight")]
         old = modules.get(path)
-        if not path or not isinstance(old, (torch.nn.Linear, torch.nn.Embedding)):
+        if not path or type(old) not in (torch.nn.Linear, torch.nn.Embedding, TokenEmbedding):
+            continue
+        if isinstance(old, torch.nn.Embedding) and old.max_norm is not None:
             continue
         w = Int4Weight.from_entry(entry, old.weight.shape[1])
         if w.shape != tuple(old.weight.shape):
@@ -382,7 +398,9 @@ def load_compressed(model: torch.nn.Module, compressed: dict) -> list[str]:
             new = Int4Linear(w, old.bias)
         else:
             new = Int4Embedding(w, old.weight.dtype)
-        parent, _, leaf = path.rpartition(".")
-        setattr(modules[parent] if parent else model, leaf, new)
+        for at in [p for p, m in modules.items() if m is old]:
+            parent, _, leaf = at.rpartition(".")
+            setattr(modules[parent], leaf, new)
+            modules[at] = new
         done.append(path)
     return done

@@ -107,6 +107,71 @@ def test_load_compressed_leaves_the_rest():
         load_compressed(torch.nn.Sequential(torch.nn.Linear(32, 17)).to(ROOT_DEV), {"0.weight": state["0.weight"]})
 
 
+def test_load_compressed_replaces_what_computes_the_same():
+    """Subclasses, an Embedding with max_norm and a module elsewhere stay; a module held twice goes in both places."""
+    from llmcompressorsharp_b200 import Int4Embedding, Int4Linear, RtnConfig, load_compressed, rtn_quantize
+
+    class Doubled(torch.nn.Linear):
+        def forward(self, x):
+            return 2 * super().forward(x)
+
+    def made(w):
+        _, c, s, z = rtn_quantize(w, RtnConfig(4, True, "channel"))
+        return {"codes": c, "scales": s, "zero_points": z, "num_bits": 4, "symmetric": True, "strategy": "channel", "group_size": 128}
+
+    m = torch.nn.ModuleDict({"a": torch.nn.Linear(32, 32), "d": Doubled(32, 32), "n": torch.nn.Embedding(9, 32, max_norm=1.0),
+                             "e": torch.nn.Embedding(9, 32)}).to(ROOT_DEV)
+    m["b"] = torch.nn.Sequential(m["a"])
+    state = {n + ".weight": made(m[n].weight) for n in ("a", "d", "n", "e")}
+    assert sorted(load_compressed(m, state)) == ["a", "e"]
+    assert type(m["d"]) is Doubled and type(m["n"]) is torch.nn.Embedding and type(m["e"]) is Int4Embedding
+    assert type(m["a"]) is Int4Linear and m["b"][0] is m["a"]
+
+
+@pytest.mark.parametrize("options", [{}, {"padding_idx": 3}, {"max_norm": 0.5}, {"scale_grad_by_freq": True}, {"dtype": torch.float64}])
+def test_token_embedding_is_torchs(options):
+    """The model's embedding keeps torch's values and gradients under each of torch's options.  Gradients are sums of
+    up to 40 terms 2^-3 k of fp32 or wider, exact in any order; a division by a count is one rounding."""
+    from llmcompressorsharp_b200.calibration import TokenEmbedding
+
+    gen = torch.Generator().manual_seed(0)
+    ours, theirs = TokenEmbedding(11, 24, device=ROOT_DEV, **options), torch.nn.Embedding(11, 24, device=ROOT_DEV, **options)
+    theirs.load_state_dict(ours.state_dict())
+    ids = torch.randint(0, 11, (4, 10), generator=gen).to(ROOT_DEV)
+    dy = (torch.randint(-8, 9, (4, 10, 24), generator=gen) * 0.125).to(ROOT_DEV, ours.weight.dtype)
+    y, z = ours(ids), theirs(ids)
+    assert torch.equal(y, z)
+    y.backward(dy)
+    z.backward(dy)
+    if options.get("scale_grad_by_freq"):
+        assert torch.allclose(ours.weight.grad, theirs.weight.grad, rtol=2 ** -20, atol=2 ** -20)
+    else:
+        assert torch.equal(ours.weight.grad, theirs.weight.grad)
+
+
+@pytest.mark.parametrize("tokens,dtype", [(1, torch.bfloat16), (100, torch.float16), (300, torch.bfloat16), (300, torch.float32)])
+def test_an_sm_limit_changes_no_result(tokens, dtype):
+    """A context's limit of SMs leaves the size of a workspace asked for before it, and every bit, as they were."""
+    from llmcompressorsharp_b200 import _lib, int4_linear
+
+    p = weight(entry(400, 640, "group", 128, True)[0], 640)
+    x = torch.randn(tokens, 640, generator=torch.Generator().manual_seed(2)).to(ROOT_DEV, dtype).requires_grad_(True)
+
+    def both():
+        y = int4_linear(x, p)
+        return y.detach(), torch.autograd.grad(y, [x], torch.ones_like(y))[0]
+
+    want = both()
+    ctx = _lib.ctx_handle(p.device.index)
+    try:
+        for limit in (1, 7):
+            _lib.call("llmc_set_sm_limit", ctx, limit)
+            for got, w in zip(both(), want):
+                assert torch.equal(got, w)
+    finally:
+        _lib.call("llmc_set_sm_limit", ctx, 0)
+
+
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 def test_quantisation_aware_embedding_under_a_frozen_packed_layer(dtype):
     """Table -> FakeQuantize (straight through) -> embedding -> packed layer; every gradient against its formula."""
