@@ -381,7 +381,7 @@ llmc_status llmc_int4_layout(llmc_ctx* ctx, void* stream, const uint8_t* codes, 
 llmc_status llmc_int4_dequantize(llmc_ctx* ctx, void* stream, const llmc_int4_weight* w, int32_t dtype, void* out,
                                  int64_t ldo);
 /* y [tokens, ldy] = x [tokens, ldx] W^T + bias (bias [rows], may be NULL), all of dtype.  Sums in fp32,
- * one rounding.  With few tokens (16 and fewer always, up to 256 for a small weight) the codes enter as
+ * one rounding.  With few tokens (32 and fewer always, up to 256 in many cases) the codes enter as
  * exact integers; with more, and in the gradient, W is rounded to a 16-bit dtype first, or kept to 24
  * bits for F32.  The sums of integers times x come before the scale: they must stay in fp32's range. */
 llmc_status llmc_int4_linear_workspace(llmc_ctx* ctx, const llmc_int4_weight* w, const void* x, int32_t dtype,

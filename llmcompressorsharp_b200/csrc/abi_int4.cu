@@ -21,13 +21,15 @@ struct DeviceScope {
 };
 
 constexpr int64_t MAX_DIM = (int64_t)1 << 30;     // rows, columns, tokens
-// Products that go to the few-row kernel, which reads the codes anew for each 16 tokens: up to 16 tokens, and more while
-// tokens / 16 x weights stays below what it passes the tensor-core kernel at.  That one takes about 9 us for any
-// product and as long for 17 tokens as for 128.  576 -> 1536 in bf16, 128 tokens: 9 us here, 13 there; 4096 -> 4096, 32: 15
-// and 14.5, 64: 23 and 16.  fp32 costs six products there and three here: 4096 -> 4096, 128: 86 here.
+// Products that go to the few-row kernel, which reads the codes anew for each 16 tokens: few tokens, and more while the
+// tensor-core kernel, which takes as long for 17 tokens as for 128, does not pass it.  us here and there, 16-bit: 4096 -> 14336,
+// 32 tokens 33 and 33, 48: 47 and 33; 4096 -> 4096, 32: 12.5 and 16.5, 64: 18.1 and 17.1; 576 -> 1536, 256: 11.5 and 20.
+// fp32 costs six products there and three here: 4096 -> 14336, 256: 373 and 489; 4096 -> 4096, 256: 114 and 127; with
+// few columns (not eight tiles) there is less to overlap: 576 -> 49152, 64: 117 and 118, 96: 172 and 122.
 bool few_rows(bool f32, int64_t tokens, int64_t rows, int64_t cols) {
-    if (tokens <= 16) return true;
-    return tokens <= (f32 ? 256 : 128) && (tokens + 15) / 16 * rows * cols <= (int64_t)1 << (f32 ? 27 : 25);
+    if (tokens <= (f32 ? 64 : 32)) return true;
+    if (tokens > 256) return false;
+    return (f32 && cols >= 8 * w4::TILE) || (tokens + 15) / 16 * rows * cols <= (int64_t)1 << (f32 ? 27 : 25);
 }
 
 llmc_status check_sizes(int64_t rows, int64_t cols, int64_t gs) {

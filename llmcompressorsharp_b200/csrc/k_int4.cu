@@ -230,10 +230,12 @@ struct FewArgs {
     int64_t ldy;
 };
 
-constexpr int FEW_WARPS = 8;  // per CTA at most
-// Tiles of the columns to a step and steps to a ring: what shared memory holds with sixteen tokens.
+// Warps to a CTA at most, and its shared memory: half an SM's, with fewer warps where it has to be (one CTA to an SM with
+// eight warps took 21.4 us for 4096 -> 14336 and 16 tokens, two with six 18.4; 14 or 16 warps for one token, no less than 8).
+constexpr int FEW_WARPS = 8, FEW_SMEM = 112 * 1024;
+// Tiles of the columns to a step and steps to a ring.
 __host__ __device__ constexpr int few_tiles(int nt, int rb) { return nt == 1 && rb == 1 ? 2 : 1; }
-__host__ __device__ constexpr int few_stages(int nt, int rb) { return nt == 2 && rb == 1 ? 5 : 3; }
+__host__ __device__ constexpr int few_stages(int nt, int rb) { return nt == 1 && rb < 4 ? 3 : 2; }
 
 __device__ __forceinline__ void copy16(void* dst, const void* src, int bytes) {  // bytes < 16: zeros for the rest
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(tc::smem_u32(dst)), "l"(src), "r"(bytes) : "memory");
@@ -448,13 +450,17 @@ llmc_status launch_few(llmc_ctx* ctx, const FewArgs& a, cudaStream_t st) {
     static std::atomic<bool> ready[64];
     const int64_t blocks = (a.v.rows + ROWS * RB - 1) / (ROWS * RB);
     const int ktiles = (int)(a.v.kp / TILE), tiles = (a.tokens + 8 * NT - 1) / (8 * NT);
-    const int steps = (ktiles + FEW_TILES - 1) / FEW_TILES, warps = steps < FEW_WARPS ? steps : FEW_WARPS, toks = a.tokens < 8 * NT ? a.tokens : 8 * NT;
-    size_t sm = 16 + (size_t)warps * STAGES * FEW_TILES * (RB * REC + (PIECES == 1 ? toks * 256 : 0)), sums = (size_t)warps * 8 * NT * ROWS * RB * sizeof(float);
+    const int steps = (ktiles + FEW_TILES - 1) / FEW_TILES, toks = a.tokens < 8 * NT ? a.tokens : 8 * NT;
+    const int each = STAGES * FEW_TILES * (RB * REC + (PIECES == 1 ? toks * 256 : 0));
+    int warps = FEW_WARPS;
+    if (warps > (FEW_SMEM - 16) / each) warps = (FEW_SMEM - 16) / each;
+    const int rounds = (steps + warps - 1) / warps;
+    warps = (steps + rounds - 1) / rounds;  // no more than finish as early
+    size_t sm = 16 + (size_t)warps * each, sums = (size_t)warps * 8 * NT * ROWS * RB * sizeof(float);
     if (sm < sums) sm = sums;
-    constexpr int MOST = 16 + FEW_WARPS * STAGES * FEW_TILES * (RB * REC + (PIECES == 1 ? 8 * NT * 256 : 0));
-    static_assert(MOST <= 227 * 1024, "shared memory of an SM");
+    static_assert(16 + 2 * STAGES * FEW_TILES * (RB * REC + (PIECES == 1 ? 8 * NT * 256 : 0)) <= FEW_SMEM, "room for two warps");
     if (ctx->device < 0 || ctx->device >= 64 || !ready[ctx->device].load(std::memory_order_relaxed)) {
-        LLMC_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, MOST));
+        LLMC_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, FEW_SMEM));
         if (ctx->device >= 0 && ctx->device < 64) ready[ctx->device].store(true, std::memory_order_relaxed);
     }
     kernel<<<dim3((unsigned)blocks, (unsigned)tiles), warps * 32, sm, st>>>(a);
@@ -467,17 +473,34 @@ template <typename T, typename O, int NT, int PIECES, int RB> llmc_status few_by
     return launch_few<T, O, NT, PIECES, 4, RB>(ctx, a, st);
 }
 
-template <typename T, typename O, int PIECES> llmc_status few_by_size(llmc_ctx* ctx, const FewArgs& a, cudaStream_t st) {
-    if constexpr (PIECES == 1) {
-        if (a.tokens > 8) {
-            // x is 256 bytes a token beside a record's 1,104: with many tokens several records share it, as long as the
-            // rows still give every SM a CTA
-            const int64_t blocks = (a.v.rows + ROWS - 1) / ROWS * ((a.tokens + 15) / 16);
-            if (blocks >= 4 * ctx->sm_count) return few_by_group<T, O, 2, PIECES, 4>(ctx, a, st);
-            if (blocks >= 2 * ctx->sm_count) return few_by_group<T, O, 2, PIECES, 2>(ctx, a, st);
-        }
+// Record rows to a CTA.  Several share x, from memory and out of shared memory, at the cost of fewer CTAs: worth it where
+// the SMs have some to spare, and (with x in two fragments or three pieces, whose rings leave few warps) where the
+// contraction gives each warp a tile.  us for 1, 2, 4 rows, 16-bit: 4096 -> 14336, 8 tokens 22.2, 16.9, 13.7, 16 tokens 29.0,
+// 23.7, 18.4; 4096 -> 4096, 8 tokens 8.4, 6.2, 8.3; 576 -> 49152, 1 token 15.9, 10.5, 9.0, 16 tokens 15.4, 17.1, 17.3.  fp32: 4096 -> 14336,
+// 8 tokens 27.6, 22.1, 20.7, 16 tokens 40.6, 37.6, 31.7; 4096 -> 4096, 8 tokens 7.7, 9.3, 10.9, 16 tokens 15.3, 10.1, 16.3;
+// 576 -> 49152, 5 tokens 12.5, 11.4, 12.8, 16 tokens 23.1, 34.2, 32.6; 576 -> 1536, 16 tokens 5.2, 4.1, 6.4.
+template <int NT, int PIECES> int few_record_rows(const llmc_ctx* ctx, const FewArgs& a) {
+    const int64_t blocks = (a.v.rows + ROWS - 1) / ROWS * ((a.tokens + 8 * NT - 1) / (8 * NT)), sms = ctx->sm_count;
+    const bool deep = a.v.kp >= 8 * TILE;
+    if (PIECES == 1) {
+        if (NT == 2 && !deep) return 1;
+        // one token: 14336 rows 12.4, 12.7, 12.8
+        return blocks >= (a.tokens > 1 ? 4 : 8) * sms ? 4 : a.tokens > 1 && 2 * blocks >= 3 * sms ? 2 : 1;
     }
-    return a.tokens > 8 ? few_by_group<T, O, 2, PIECES, 1>(ctx, a, st) : few_by_group<T, O, 1, PIECES, 1>(ctx, a, st);
+    if (NT == 1) return blocks < 4 * sms ? 1 : deep ? 4 : 2;
+    if (!deep) return blocks < 3 * sms ? 2 : 1;
+    return blocks < 6 * sms ? 2 : 4;
+}
+
+template <typename T, typename O, int NT, int PIECES> llmc_status few_by_rows(llmc_ctx* ctx, const FewArgs& a, cudaStream_t st) {
+    const int rb = few_record_rows<NT, PIECES>(ctx, a);
+    if (rb == 4) return few_by_group<T, O, NT, PIECES, 4>(ctx, a, st);
+    if (rb == 2) return few_by_group<T, O, NT, PIECES, 2>(ctx, a, st);
+    return few_by_group<T, O, NT, PIECES, 1>(ctx, a, st);
+}
+
+template <typename T, typename O, int PIECES> llmc_status few_by_size(llmc_ctx* ctx, const FewArgs& a, cudaStream_t st) {
+    return a.tokens > 8 ? few_by_rows<T, O, 2, PIECES>(ctx, a, st) : few_by_rows<T, O, 1, PIECES>(ctx, a, st);
 }
 
 }  // namespace

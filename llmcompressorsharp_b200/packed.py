@@ -221,7 +221,7 @@ class _Int4LinearFn(torch.autograd.Function):
 def int4_linear(x: torch.Tensor, weight: Int4Weight, bias: torch.Tensor | None = None) -> torch.Tensor:
     """y = x W^T + bias for x [..., cols] of float32, bfloat16 or float16; y [..., rows] of x's type.
 
-    Sums are fp32 and rounded once.  With few rows of x (16 and fewer always, up to 256 for a small weight) the
+    Sums are fp32 and rounded once.  With few rows of x (32 and fewer always, up to 256 in many cases) the
     codes are multiplied as exact integers; with more, and in the backward pass, W is rounded to x's 16-bit
     type first (as a dequantised weight of that type is), or kept to 24 bits for float32.  Differentiable once,
     in x and the bias."""

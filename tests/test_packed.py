@@ -162,7 +162,7 @@ def test_layout_reads_back(m, n, strategy, group, sym, bits):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("strategy,group,sym,bits", GRIDS)
-@pytest.mark.parametrize("tokens", [1, 8, 9, 16, 17, 129])
+@pytest.mark.parametrize("tokens", [1, 8, 9, 16, 17, 129, 257])
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
 def test_products_of_exact_numbers_are_exact(tokens, dtype, strategy, group, sym, bits):
     """Also at the joins of 128 rows and columns, with and without a bias, and for the gradients."""

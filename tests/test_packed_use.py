@@ -131,7 +131,9 @@ def test_load_compressed_replaces_what_computes_the_same():
 @pytest.mark.parametrize("options", [{}, {"padding_idx": 3}, {"max_norm": 0.5}, {"scale_grad_by_freq": True}, {"dtype": torch.float64}])
 def test_token_embedding_is_torchs(options):
     """The model's embedding keeps torch's values and gradients under each of torch's options.  Gradients are sums of
-    up to 40 terms 2^-3 k of fp32 or wider, exact in any order; a division by a count is one rounding."""
+    up to 40 terms 2^-3 k of fp32 or wider, exact in any order; a division by a count is one rounding.  With max_norm
+    both sides are torch's, which adds a row's 24 squares in no fixed order: a relative 23 x 2^-24 at most, half of it
+    in the root, and with the root's, the quotient's and the product's roundings less than 2^-20 on each side."""
     from llmcompressorsharp_b200.calibration import TokenEmbedding
 
     gen = torch.Generator().manual_seed(0)
@@ -140,7 +142,10 @@ def test_token_embedding_is_torchs(options):
     ids = torch.randint(0, 11, (4, 10), generator=gen).to(ROOT_DEV)
     dy = (torch.randint(-8, 9, (4, 10, 24), generator=gen) * 0.125).to(ROOT_DEV, ours.weight.dtype)
     y, z = ours(ids), theirs(ids)
-    assert torch.equal(y, z)
+    if options.get("max_norm"):
+        assert torch.allclose(y, z, rtol=2 ** -19, atol=0)
+    else:
+        assert torch.equal(y, z)
     y.backward(dy)
     z.backward(dy)
     if options.get("scale_grad_by_freq"):
@@ -202,7 +207,7 @@ def test_quantisation_aware_embedding_under_a_frozen_packed_layer(dtype):
     assert bool(((table.grad.double().cpu() - want).abs() <= bound).all())
 
 
-@pytest.mark.parametrize("tokens", [1, 5, 16, 40, 200])
+@pytest.mark.parametrize("tokens", [1, 5, 16, 40, 200, 300])
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 def test_captured_graphs_of_one_weight(tokens, dtype):
     """Two graphs of the same weight at once, replayed with new inputs on two streams: forward, and forward with backward."""
@@ -343,7 +348,7 @@ def test_non_finite_gradients_stay_in_their_row(dtype):
     assert bool(got[3][v == 0].isnan().all()) and bool((got[3][v > 0] == float("inf")).all()) and bool((got[3][v < 0] == -float("inf")).all())
 
 
-@pytest.mark.parametrize("tokens,dtype", [(200, torch.bfloat16), (300, torch.float16), (300, torch.float32)])
+@pytest.mark.parametrize("tokens,dtype", [(300, torch.bfloat16), (300, torch.float16), (300, torch.float32)])
 def test_a_wait_that_gives_up_is_reported_and_passes(tokens, dtype):
     """The limit of 0 makes the tensor-core kernel give up at its first wait, before it has issued a copy."""
     from llmcompressorsharp_b200 import _lib
