@@ -418,12 +418,15 @@ llmc_status lookup(llmc_ctx* ctx, cudaStream_t st, const void* table, int64_t ld
     return check_launch(ctx, "embedding");
 }
 
-// The sort's largest cluster: sixteen where the device places such a cluster, else the portable eight.
-int largest_cluster(int device, const void* fn, size_t sm) {
-    static std::atomic<int> known[64];
-    if (device < 0 || device >= 64) return 8;
-    int n = known[device].load(std::memory_order_relaxed);
-    if (n) return n;
+// Readies the sort on a device, once, and gives its largest cluster: sixteen where the device places such a cluster, else
+// the portable eight.
+llmc_status ready_sort(int device, int ids64, const void* fn, size_t sm, int& n) {
+    static std::atomic<int> known[2][64];
+    const bool keep = device >= 0 && device < 64;
+    n = keep ? known[ids64 ? 1 : 0][device].load(std::memory_order_relaxed) : 0;
+    if (n) return LLMC_OK;
+    LLMC_CUDA_TRY(cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sm));
+    LLMC_CUDA_TRY(cudaFuncSetAttribute(fn, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(16);
     cfg.blockDim = dim3(SORT_NT);
@@ -438,8 +441,8 @@ int largest_cluster(int device, const void* fn, size_t sm) {
     const bool ok = cudaOccupancyMaxActiveClusters(&clusters, fn, &cfg) == cudaSuccess && clusters > 0;
     if (!ok) cudaGetLastError();
     n = ok ? 16 : 8;
-    known[device].store(n, std::memory_order_relaxed);
-    return n;
+    if (keep) known[ids64 ? 1 : 0][device].store(n, std::memory_order_relaxed);
+    return LLMC_OK;
 }
 
 size_t carve(Plan& p, void* ws, int64_t tokens, int64_t vocab, int64_t hidden) {
@@ -501,9 +504,8 @@ llmc_status embedding_grad(llmc_ctx* ctx, cudaStream_t st, const void* ids, int 
     const int passes = (width + DIGIT - 1) / DIGIT, bits = (width + passes - 1) / passes;
     const size_t sm = (size_t)SORT_WARPS * BINS * sizeof(uint32_t);
     const void* fn = ids64 ? (const void*)sort_kernel<int64_t> : (const void*)sort_kernel<int32_t>;
-    LLMC_CUDA_TRY(cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sm));
-    LLMC_CUDA_TRY(cudaFuncSetAttribute(fn, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
-    const int most = largest_cluster(ctx->device, fn, sm);
+    int most = 0;
+    LLMC_TRY(ready_sort(ctx->device, ids64, fn, sm, most));
     int ctas = 1;  // about 2,048 tokens to a CTA
     while (ctas < most && (int64_t)ctas * 2048 < tokens) ctas *= 2;
     cudaLaunchConfig_t cfg = {};

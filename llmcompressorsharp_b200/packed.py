@@ -203,6 +203,12 @@ def _col_sum(x2: torch.Tensor) -> torch.Tensor:
     return out
 
 
+def _once(backward):
+    """once_differentiable, whose wrapping a pass that records no graph goes without."""
+    guarded = once_differentiable(backward)
+    return lambda ctx_, dy: guarded(ctx_, dy) if torch.is_grad_enabled() else backward(ctx_, dy)
+
+
 class _Int4LinearFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx_, x, weight, bias):
@@ -210,7 +216,7 @@ class _Int4LinearFn(torch.autograd.Function):
         return weight._product(x, bias, False)
 
     @staticmethod
-    @once_differentiable
+    @_once
     def backward(ctx_, dy):
         w = ctx_.weight
         dx = w._product(dy, None, True) if ctx_.needs_input_grad[0] else None
@@ -264,17 +270,16 @@ class _EmbeddingFn(torch.autograd.Function):
         return _lookup(ids, table, scale)
 
     @staticmethod
-    @once_differentiable
+    @_once
     def backward(ctx_, dy):
         (ids,) = ctx_.saved_tensors
         vocab, hidden = ctx_.shape
         d2 = _rows(dy, hidden)
-        flat = ids.reshape(-1)
         index = dy.device.index
         ctx = _lib.ctx_handle(index)
-        ws = _scratch("llmc_embedding_grad_workspace", index, dy.device, flat.numel(), vocab, hidden)
+        ws = _scratch("llmc_embedding_grad_workspace", index, dy.device, ids.numel(), vocab, hidden)
         out = torch.empty(vocab, hidden, dtype=dy.dtype, device=dy.device)
-        _lib.call("llmc_embedding_grad", ctx, _lib.stream(index), flat.data_ptr(), int(flat.dtype == torch.int64), flat.numel(),
+        _lib.call("llmc_embedding_grad", ctx, _lib.stream(index), ids.data_ptr(), int(ids.dtype == torch.int64), ids.numel(),
                   d2.data_ptr(), _DTYPES[dy.dtype], _pitch(d2), vocab, hidden, ctx_.scale, ctx_.padding, out.data_ptr(),
                   ws.data_ptr(), ws.numel())
         return out, None, None, None
