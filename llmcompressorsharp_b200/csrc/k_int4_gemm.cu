@@ -27,10 +27,11 @@
 // A stage is a whole tile, 128 of the contraction: the MMA warp's two waits and its commit take some hundreds of
 // clocks, which the MMAs of 64 (512 clocks) did not cover.
 //
-// 4096 -> 14336, 8,192 tokens, bf16: 731 us, 1.32 PFLOP/s, which is what the power limit leaves a large product of the
-// library's too (0.94 of its sustained rate); 813 with one thread issuing the MMAs inside a branch and building its
-// descriptors each time.  2,048 tokens of 4096 -> 4096: 71 to 84 us, and its gradient the same.  At 17 to 128 tokens
-// the eight warps that dequantise bound it: 29 us for 4096 -> 14336, where the codes alone are read in 5.
+// 4096 -> 14336, 8,192 tokens, bf16: 735 to 760 us in short runs (1.3 PFLOP/s; the library's product of a 16-bit weight 648),
+// 860 back to back at the power limit (731); 813 in short runs with one thread issuing the MMAs inside a branch and
+// building its descriptors each time.  2,048 tokens of 4096 -> 4096: 68 us back to back (53), its gradient 66.  At 33 to 128
+// tokens the eight warps that dequantise bound it: 29 us for 4096 -> 14336, where the codes alone are read in 5.  Numbers
+// made before the wait for a free stage instead of behind it: no faster.
 // Every wait is bounded.
 #include "int4.cuh"
 #include "ops.h"
