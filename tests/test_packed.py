@@ -222,6 +222,32 @@ def test_products_of_few_tokens_on_the_tensor_cores(dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("m,n,tokens", [(19001, 130, 1), (3601, 130, 5), (9601, 130, 7), (9601, 1100, 8), (4801, 1100, 12), (4801, 1100, 32),
+                                        (4801, 1100, 48), (601, 1030, 250), (9601, 70, 30)])
+@pytest.mark.parametrize("group", [32, 64, 130])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+def test_rows_that_share_x_are_exact(m, n, tokens, dtype, group):
+    """Weights of enough rows for each number of record rows to a CTA, the last of them partly past the weight; sums of
+    1,100 terms of at most 60 in steps of 2^-6 are exact in fp32."""
+    from llmcompressorsharp_b200 import _lib, int4_linear
+
+    code = _lib.dtype_code(dtype)
+    e, w = entry(m, n, group=group, pow2=True, seed=m, device=ROOT_DEV)
+    g = torch.Generator().manual_seed(tokens)
+    x = torch.randint(-4, 5, (tokens, n), generator=g).double()
+    b = torch.randint(-4, 5, (m,), generator=g).double()
+    p = weight(e, n)
+    assert torch.equal(int4_linear(x.to(ROOT_DEV, dtype), p, b.to(ROOT_DEV, dtype)).cpu(), (x @ w.t() + b).float().to(dtype))
+    y = torch.full((tokens + 1, m + 3), 7.0, dtype=dtype, device=ROOT_DEV)
+    xd = x.to(ROOT_DEV, dtype)
+    ws = p._workspace("llmc_int4_linear_workspace", xd.data_ptr(), code, tokens, n)
+    _lib.call("llmc_int4_linear", p._ctx, _lib.stream(0), p._ref, xd.data_ptr(), code, tokens, n, None, y.data_ptr(), m + 3,
+              ws.data_ptr() if ws is not None else None, ws.numel() if ws is not None else 0)
+    assert torch.equal(y[:tokens, :m].cpu(), (x @ w.t()).float().to(dtype))
+    assert bool((y[tokens:] == 7).all()) and bool((y[:, m:] == 7).all())
+
+
+@pytest.mark.gpu
 def test_gradient_against_differences():
     """The product is linear in x: a step of t along d changes it by t (d W^T), whatever x is."""
     from llmcompressorsharp_b200 import int4_linear
