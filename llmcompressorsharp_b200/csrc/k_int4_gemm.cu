@@ -465,8 +465,6 @@ __global__ void __launch_bounds__(32 * (3 + (PIECES == 3 ? 8 : 4) + DQ_WARPS), 1
                     for (int c = 0; c < GROUPS; c++)
                         sc[i][c].set(scales[slot_of(c, ng)] * e[DIR == 0 ? i : c], zeros[slot_of(c, ng)]);
                 }
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&cempty[cs]);
                 if (!mbar_wait(&empty[sg], ph ^ 1u, abort_flag, a.err, a.wait_limit)) return false;
                 unsigned char* b = smem + sg * STAGE_BYTES + A_BYTES;
 #pragma unroll
@@ -487,6 +485,10 @@ __global__ void __launch_bounds__(32 * (3 + (PIECES == 3 ? 8 : 4) + DQ_WARPS), 1
                 if (lane == 0) {
                     if constexpr (CG == 2) mbar_arrive_cluster_cta(mapa_shared(smem_u32(&bfull[sg]), 0));
                     else mbar_arrive(&bfull[sg]);
+                    // The tile of codes is let go of only now, when what was read of it has gone into the stores above: let
+                    // go of right after the loads, it was refilled too early at times beside another stream's product
+                    // (fp32 gradients, some of 1,256 tiles in most runs).
+                    mbar_arrive(&cempty[cs]);
                 }
                 return true;
             });

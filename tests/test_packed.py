@@ -248,6 +248,27 @@ def test_rows_that_share_x_are_exact(m, n, tokens, dtype, group):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("tokens,m,n", [(1300, 1801, 260), (1300, 260, 1801), (2100, 1801, 1030)])
+@pytest.mark.parametrize("group", [32, 64, 100, 128])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_products_of_many_tiles_are_exact(tokens, m, n, dtype, group):
+    """More tiles of 128 x 128 than SMs in the product, its gradient or both, the last ones ragged.  Sums of up to 1,801
+    terms below 8 in steps of 2^-6 are exact in fp32."""
+    from llmcompressorsharp_b200 import int4_linear
+
+    e, w = entry(m, n, group=group, pow2=True, seed=m, device=ROOT_DEV)
+    g = torch.Generator().manual_seed(tokens)
+    x = torch.randint(-4, 5, (tokens, n), generator=g).double()
+    b = torch.randint(-4, 5, (m,), generator=g).double()
+    dy = torch.randint(-4, 5, (tokens, m), generator=g).double()
+    xd = x.to(ROOT_DEV, dtype).requires_grad_(True)
+    wd = w.to(ROOT_DEV)
+    y = int4_linear(xd, weight(e, n), b.to(ROOT_DEV, dtype))
+    assert torch.equal(y, (x.to(ROOT_DEV) @ wd.t() + b.to(ROOT_DEV)).float().to(dtype))
+    assert torch.equal(torch.autograd.grad(y, xd, dy.to(ROOT_DEV, dtype))[0], (dy.to(ROOT_DEV) @ wd).float().to(dtype))
+
+
+@pytest.mark.gpu
 def test_gradient_against_differences():
     """The product is linear in x: a step of t along d changes it by t (d W^T), whatever x is."""
     from llmcompressorsharp_b200 import int4_linear

@@ -207,7 +207,7 @@ def test_quantisation_aware_embedding_under_a_frozen_packed_layer(dtype):
     assert bool(((table.grad.double().cpu() - want).abs() <= bound).all())
 
 
-@pytest.mark.parametrize("tokens", [1, 5, 16, 40, 200, 300])
+@pytest.mark.parametrize("tokens", [1, 5, 16, 40, 200, 300, 20000])
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 def test_captured_graphs_of_one_weight(tokens, dtype):
     """Two graphs of the same weight at once, replayed with new inputs on two streams: forward, and forward with backward."""
@@ -253,6 +253,26 @@ def test_captured_graphs_of_one_weight(tokens, dtype):
         for i in range(2):
             for a, b in zip(outs[i], step(i)):
                 assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("tokens", [400, 20000])
+def test_products_on_two_streams_at_once(tokens, dtype):
+    """Two streams of products share the SMs and give, tile by tile, the bits that each gives alone."""
+    p = weight(entry(300, 1000, group=128, device=ROOT_DEV)[0], 1000)
+    g = torch.Generator().manual_seed(tokens)
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for back, n in ((True, 300), (False, 1000)):
+        src = [torch.randn(tokens, n, generator=g).to(ROOT_DEV, dtype) for _ in range(2)]
+        want = [p._product(a, None, back) for a in src]
+        torch.cuda.synchronize()
+        for _ in range(12):
+            got = []
+            for i in (0, 1, 0, 1):
+                with torch.cuda.stream(streams[i]):
+                    got.append((i, p._product(src[i], None, back)))
+            torch.cuda.synchronize()
+            assert all(torch.equal(y, want[i]) for i, y in got)
 
 
 def test_first_calls_inside_a_capture():
@@ -348,8 +368,9 @@ def test_non_finite_gradients_stay_in_their_row(dtype):
     assert bool(got[3][v == 0].isnan().all()) and bool((got[3][v > 0] == float("inf")).all()) and bool((got[3][v < 0] == -float("inf")).all())
 
 
-@pytest.mark.parametrize("tokens,dtype", [(300, torch.bfloat16), (300, torch.float16), (300, torch.float32)])
-def test_a_wait_that_gives_up_is_reported_and_passes(tokens, dtype):
+@pytest.mark.parametrize("tokens,m,k,dtype", [(300, 300, 256, torch.bfloat16), (300, 300, 256, torch.float16), (300, 300, 256, torch.float32),
+                                              (1300, 1801, 1792, torch.bfloat16), (1300, 1801, 1792, torch.float16)])
+def test_a_wait_that_gives_up_is_reported_and_passes(tokens, m, k, dtype):
     """The limit of 0 makes the tensor-core kernel give up at its first wait, before it has issued a copy."""
     from llmcompressorsharp_b200 import _lib
 
@@ -357,13 +378,13 @@ def test_a_wait_that_gives_up_is_reported_and_passes(tokens, dtype):
     ctx = C.c_void_p()
     assert lib.llmc_init(0, C.byref(ctx)) == 0
     try:
-        e, _ = entry(300, 256, group=64, device=ROOT_DEV)
-        p = weight(e, 256)
-        x = torch.randn(tokens, 256, generator=torch.Generator().manual_seed(0)).to(ROOT_DEV, dtype)
-        dy = torch.randn(tokens, 300, generator=torch.Generator().manual_seed(1)).to(ROOT_DEV, dtype)
+        e, _ = entry(m, k, group=64, device=ROOT_DEV)
+        p = weight(e, k)
+        x = torch.randn(tokens, k, generator=torch.Generator().manual_seed(0)).to(ROOT_DEV, dtype)
+        dy = torch.randn(tokens, m, generator=torch.Generator().manual_seed(1)).to(ROOT_DEV, dtype)
         torch.cuda.synchronize()
         for back in (False, True):
-            a, n = (dy, 256) if back else (x, 300)
+            a, n = (dy, k) if back else (x, m)
             want = p._product(a, None, back)
             out = torch.empty(tokens, n, dtype=dtype, device=ROOT_DEV)
             need = C.c_int64()
