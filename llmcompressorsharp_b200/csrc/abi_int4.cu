@@ -23,7 +23,7 @@ struct DeviceScope {
 constexpr int64_t MAX_DIM = (int64_t)1 << 30;     // rows, columns, tokens
 // Products that go to the few-row kernel, which reads the codes anew for each 16 tokens: few tokens, and more while the
 // tensor-core kernel, which takes as long for 17 tokens as for 128, does not pass it.  us here and there, 16-bit: 4096 -> 14336,
-// 32 tokens 33 and 33, 48: 47 and 33; 4096 -> 4096, 32: 12.5 and 16.5, 64: 18.1 and 17.1; 576 -> 1536, 256: 11.5 and 20.
+// 32 tokens 33 and 33, 48: 47 and 33; 4096 -> 4096, 32: 12.5 and 16.5, 64: 18.1 and 17.1; 576 -> 1536, 256: 11.5 and 14.
 // fp32 costs six products there and three here: 4096 -> 14336, 256: 373 and 489; 4096 -> 4096, 256: 114 and 127; with
 // few columns (not eight tiles) there is less to overlap: 576 -> 49152, 64: 117 and 118, 96: 172 and 122.
 bool few_rows(bool f32, int64_t tokens, int64_t rows, int64_t cols) {

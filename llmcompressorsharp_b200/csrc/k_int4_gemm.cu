@@ -20,8 +20,8 @@
 // accumulation truncates, so TMEM then holds 256 terms of the contraction at most before the epilogue adds them
 // to fp32 registers.
 //
-// A persistent grid of CTA pairs (256 tokens x 256 columns, cta_group::2) or, for up to 128 tokens and for fp32,
-// single CTAs (128 x 128).  Per CTA: a TMA warp for the activations and one for the codes (a tile of 128 x 128
+// A persistent grid of CTA pairs (256 tokens x 256 columns, cta_group::2) or, for products that a round of them holds and
+// for fp32, single CTAs (128 x 128).  Per CTA: a TMA warp for the activations and one for the codes (a tile of 128 x 128
 // weights in one bulk copy), an MMA warp, epilogue warps, eight dequantising warps, a ring of
 // STAGES x (32 KB activations + 32 KB weights) and one of CODE_STAGES tiles of codes, two accumulators in TMEM.
 // A stage is a whole tile, 128 of the contraction: the MMA warp's two waits and its commit take some hundreds of
@@ -622,13 +622,20 @@ llmc_status launch(llmc_ctx* ctx, cudaStream_t st, const CUtensorMap& map, GemmI
 
 }  // namespace
 
-// CTAs per tile for a product of this many tokens and columns.
-int int4_gemm_cg(int dtype, int64_t tokens, int64_t cols) { return dtype != LLMC_DTYPE_F32 && tokens > 128 && cols > 128 ? 2 : 1; }
+// CTAs per tile: pairs (256 x 256) share what they dequantise and load, single CTAs (128 x 128) fill more SMs, so they are
+// taken while one round of them holds the product and the contraction is not so long that sharing counts for more.  us, fp16,
+// single and pairs: 4096 -> 4096, 512 tokens (128 tiles) 33 and 38, 768 (192) 54 and 41; 2048 -> 2048, 1,024 (128) 21 and 32,
+// 2,048 (256) 34 and 29; 576 -> 1536, 1,024 (96) 12 and 25; 14336 -> 4096, 160 tokens 52 and 42, 512 86 and 76.
+int int4_gemm_cg(const llmc_ctx* ctx, int dtype, int64_t tokens, int64_t cols, int64_t contraction) {
+    if (dtype == LLMC_DTYPE_F32 || tokens <= 128 || cols <= 128) return 1;
+    const bool round = (tokens + 127) / 128 * ((cols + 127) / 128) <= ctx->sm_count;
+    return round && contraction <= 64 * TILE ? 1 : 2;
+}
 
 // Splits of the contraction: enough to give every worker a tile, two tiles of 128 to a split at least (one in fp32,
 // where a tile is six products).
 int int4_gemm_splits(const llmc_ctx* ctx, int dtype, int64_t tokens, int64_t cols, int64_t contraction) {
-    const int cg = int4_gemm_cg(dtype, tokens, cols);
+    const int cg = int4_gemm_cg(ctx, dtype, tokens, cols, contraction);
     const int64_t tile = 128 * cg, tiles = ((tokens + tile - 1) / tile) * ((cols + tile - 1) / tile);
     // by the device's SMs, not llmc_set_sm_limit's: a workspace that was asked for stays large enough
     const int64_t kt = contraction / TILE, workers = ctx->sm_count / cg;
@@ -648,7 +655,7 @@ llmc_status int4_gemm(llmc_ctx* ctx, cudaStream_t st, const w4::View& v, int dir
     if (!enc) return fail(LLMC_ERR_CUDA, "cuTensorMapEncodeTiled is not available");
     const int pieces = dtype == LLMC_DTYPE_F32 ? 4 : 1;
     const int64_t cols = dir == 0 ? v.rows : v.kp, contraction = dir == 0 ? v.kp : v.mp;
-    const int cg = int4_gemm_cg(dtype, tokens, cols);
+    const int cg = int4_gemm_cg(ctx, dtype, tokens, cols, contraction);
     GemmInt4 g{};
     g.v = v;
     g.tokens = tokens;
