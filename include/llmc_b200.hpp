@@ -89,6 +89,33 @@ inline void CheckCuda(cudaError_t e, const char* what) {
     if (e != cudaSuccess) throw LlmcException(LLMC_ERR_CUDA, std::string(what) + ": " + cudaGetErrorString(e));
 }
 
+namespace detail {
+inline int CurrentDevice() {
+    int d = 0;
+    CheckCuda(cudaGetDevice(&d), "cudaGetDevice");
+    return d;
+}
+
+// Every copy of this header: ordered after all work in flight on `device`, and complete when it returns.  Contexts
+// run on non-blocking streams, which the legacy stream that cudaMemcpy uses neither waits for nor holds up: without
+// the first wait a read-back may find what the memory held before, without the second a kernel may read its input
+// (a small pageable one is staged, a device-to-device one only queued, when cudaMemcpy returns) before it is there.
+inline void Copy(int device, void* dst, const void* src, size_t bytes, cudaMemcpyKind kind) {
+    if (bytes == 0) return;
+    const int current = CurrentDevice();
+    struct Back {
+        int device;
+        ~Back() {
+            if (device >= 0) cudaSetDevice(device);
+        }
+    } back{current != device ? current : -1};
+    if (current != device) CheckCuda(cudaSetDevice(device), "cudaSetDevice");
+    CheckCuda(cudaDeviceSynchronize(), "cudaDeviceSynchronize");
+    CheckCuda(cudaMemcpy(dst, src, bytes, kind), "cudaMemcpy");
+    if (kind != cudaMemcpyDeviceToHost) CheckCuda(cudaStreamSynchronize(cudaStreamLegacy), "cudaStreamSynchronize");
+}
+}  // namespace detail
+
 // ---- device context ---------------------------------------------------------------------------
 class Context {
    public:
@@ -133,6 +160,7 @@ class DeviceTensor {
    public:
     DeviceTensor() = default;
     DeviceTensor(std::vector<int64_t> shape, DType dtype) : shape_(std::move(shape)), dtype_(dtype) {
+        device_ = detail::CurrentDevice();
         if (bytes()) CheckCuda(cudaMalloc(&data_, bytes()), "cudaMalloc");
     }
     // Host values converted to `dtype` (round to nearest even).
@@ -150,12 +178,12 @@ class DeviceTensor {
                 std::memcpy(&raw[2 * i], &h, 2);
             }
         }
-        if (t.bytes()) CheckCuda(cudaMemcpy(t.data_, raw.data(), t.bytes(), cudaMemcpyHostToDevice), "cudaMemcpy");
+        detail::Copy(t.device_, t.data_, raw.data(), t.bytes(), cudaMemcpyHostToDevice);
         return t;
     }
     std::vector<float> ToHost() const {
         std::vector<unsigned char> raw(bytes());
-        if (bytes()) CheckCuda(cudaMemcpy(raw.data(), data_, bytes(), cudaMemcpyDeviceToHost), "cudaMemcpy");
+        detail::Copy(device_, raw.data(), data_, bytes(), cudaMemcpyDeviceToHost);
         std::vector<float> out((size_t)numel());
         for (size_t i = 0; i < out.size(); i++) {
             if (dtype_ == DType::Float32) std::memcpy(&out[i], &raw[4 * i], 4);
@@ -181,6 +209,7 @@ class DeviceTensor {
             data_ = o.data_;
             shape_ = std::move(o.shape_);
             dtype_ = o.dtype_;
+            device_ = o.device_;
             o.data_ = nullptr;
         }
         return *this;
@@ -189,6 +218,7 @@ class DeviceTensor {
     DeviceTensor& operator=(const DeviceTensor&) = delete;
 
     void* data() const { return data_; }
+    int device() const { return device_; }
     DType dtype() const { return dtype_; }
     const std::vector<int64_t>& shape() const { return shape_; }
     int64_t dim() const { return (int64_t)shape_.size(); }
@@ -204,6 +234,7 @@ class DeviceTensor {
     void* data_ = nullptr;
     std::vector<int64_t> shape_;
     DType dtype_ = DType::Float32;
+    int device_ = 0;  // where data_ is
 };
 
 // ---- HessianAccumulator ------------------------------------------------------------------------
@@ -342,7 +373,7 @@ inline QuantizationParameters Affine(Context& ctx, const DeviceTensor& mins, con
                              static_cast<int32_t*>(z.data())));
     QuantizationParameters p{s.ToHost(), {}, st};
     std::vector<int32_t> zi((size_t)count);
-    CheckCuda(cudaMemcpy(zi.data(), z.data(), (size_t)count * 4, cudaMemcpyDeviceToHost), "cudaMemcpy");
+    Copy(z.device(), zi.data(), z.data(), (size_t)count * 4, cudaMemcpyDeviceToHost);
     p.ZeroPoint.assign(zi.begin(), zi.end());
     return p;
 }
@@ -357,8 +388,8 @@ class MinMaxObserver {
         if (x.numel() == 0) return;
         if (!has_) {
             const float init[2] = {std::numeric_limits<float>::infinity(), -std::numeric_limits<float>::infinity()};
-            CheckCuda(cudaMemcpy(mn_.data(), &init[0], 4, cudaMemcpyHostToDevice), "cudaMemcpy");
-            CheckCuda(cudaMemcpy(mx_.data(), &init[1], 4, cudaMemcpyHostToDevice), "cudaMemcpy");
+            detail::Copy(mn_.device(), mn_.data(), &init[0], 4, cudaMemcpyHostToDevice);
+            detail::Copy(mx_.device(), mx_.data(), &init[1], 4, cudaMemcpyHostToDevice);
         }
         Check(llmc_observer_minmax(ctx_->get(), x.data(), (int32_t)x.dtype(), x.numel() / x.last(), x.last(), x.last(),
                                    LLMC_STRATEGY_TENSOR, x.last(), static_cast<float*>(mn_.data()),
@@ -386,7 +417,7 @@ class MSEObserver {
     }
     void Update(const DeviceTensor& x) {
         DeviceTensor copy({x.numel()}, x.dtype());
-        if (x.bytes()) CheckCuda(cudaMemcpy(copy.data(), x.data(), x.bytes(), cudaMemcpyDeviceToDevice), "cudaMemcpy");
+        detail::Copy(x.device(), copy.data(), x.data(), x.bytes(), cudaMemcpyDeviceToDevice);
         samples_.push_back(std::move(copy));
     }
     QuantizationParameters GetQuantParams(int numBits, bool symmetric) {
@@ -403,9 +434,7 @@ class MSEObserver {
             joined = DeviceTensor({n}, samples_[0].dtype());
             size_t off = 0;
             for (const auto& t : samples_) {
-                if (t.bytes())
-                    CheckCuda(cudaMemcpy(static_cast<char*>(joined.data()) + off, t.data(), t.bytes(),
-                                         cudaMemcpyDeviceToDevice), "cudaMemcpy");
+                detail::Copy(t.device(), static_cast<char*>(joined.data()) + off, t.data(), t.bytes(), cudaMemcpyDeviceToDevice);
                 off += t.bytes();
             }
             flat = &joined;
@@ -490,13 +519,12 @@ class Int4PackedTensor {
         if ((int64_t)packed.size() != (elementCount + 1) / 2)
             throw ArgumentException("packed length must be (elementCount + 1) / 2");
         Int4PackedTensor t(&ctx, elementCount, scale, zeroPoint, symmetric);
-        if (!packed.empty())
-            CheckCuda(cudaMemcpy(t.packed_.data(), packed.data(), packed.size(), cudaMemcpyHostToDevice), "cudaMemcpy");
+        detail::Copy(t.packed_.device(), t.packed_.data(), packed.data(), packed.size(), cudaMemcpyHostToDevice);
         return t;
     }
     std::vector<uint8_t> PackedBytes() const {
         std::vector<uint8_t> b((size_t)((n_ + 1) / 2));
-        if (!b.empty()) CheckCuda(cudaMemcpy(b.data(), packed_.data(), b.size(), cudaMemcpyDeviceToHost), "cudaMemcpy");
+        detail::Copy(packed_.device(), b.data(), packed_.data(), b.size(), cudaMemcpyDeviceToHost);
         return b;
     }
     int64_t ElementCount() const { return n_; }
@@ -523,6 +551,7 @@ class Int4PackedTensor {
 class DeviceBytes {
    public:
     explicit DeviceBytes(size_t n) : n_(n) {
+        device_ = detail::CurrentDevice();
         if (n_) CheckCuda(cudaMalloc(&data_, n_), "cudaMalloc");
     }
     ~DeviceBytes() {
@@ -535,13 +564,14 @@ class DeviceBytes {
     template <typename T>
     std::vector<T> ToHost() const {
         std::vector<T> out(n_ / sizeof(T));
-        if (n_) CheckCuda(cudaMemcpy(out.data(), data_, out.size() * sizeof(T), cudaMemcpyDeviceToHost), "cudaMemcpy");
+        detail::Copy(device_, out.data(), data_, out.size() * sizeof(T), cudaMemcpyDeviceToHost);
         return out;
     }
 
    private:
     void* data_ = nullptr;
     size_t n_;
+    int device_ = 0;
 };
 
 // ---- RTN (RtnModifier.cs:44-122 for one weight) -----------------------------------------------
