@@ -19,6 +19,7 @@ from __future__ import annotations
 import ctypes as C
 
 import torch
+import torch.autograd.forward_ad as forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _lib
@@ -47,6 +48,31 @@ def _rows(t: torch.Tensor, last: int) -> torch.Tensor:
 def _pitch(t: torch.Tensor) -> int:
     """Elements between rows (of at most one row: its length, whatever stride torch keeps)."""
     return t.stride(0) if t.shape[0] > 1 else max(1, t.shape[1])
+
+
+def _seen_by_torch(*tensors) -> str | None:
+    """What of torch's watches the operators that are run on these tensors, if anything does: a trace of the library's
+    calls would hold empty tensors in place of their results, a transform would lose its part of them."""
+    if torch._C._is_tracing():
+        return "torch.jit's tracing"
+    if torch._C._functorch.peek_interpreter_stack() is not None:
+        if any(isinstance(t, torch.Tensor) and torch._C._functorch.is_functorch_wrapped_tensor(t) for t in tensors):
+            return "a torch.func transform"
+    if torch._C._len_torch_dispatch_stack() and torch._C._get_dispatch_mode(torch._C._TorchDispatchModeKey.PROXY) is not None:
+        return "torch.fx's tracing"
+    for t in tensors:
+        if isinstance(t, torch.Tensor) and type(t) is not torch.Tensor and type(t) is not torch.nn.Parameter:
+            from torch._subclasses import FakeTensor
+
+            if isinstance(t, FakeTensor):
+                return "a FakeTensor"
+    return None
+
+
+def _refuse_unseen(name: str, *tensors):
+    what = _seen_by_torch(*tensors)
+    if what is not None:
+        raise NotSupportedError(f"{name} cannot run under {what}: its kernels are not torch operators")
 
 
 class Int4Weight:
@@ -230,11 +256,12 @@ def int4_linear(x: torch.Tensor, weight: Int4Weight, bias: torch.Tensor | None =
     Sums are fp32 and rounded once.  With few rows of x (32 and fewer always, up to 256 in many cases) the
     codes are multiplied as exact integers; with more, and in the backward pass, W is rounded to x's 16-bit
     type first (as a dequantised weight of that type is), or kept to 24 bits for float32.  Differentiable once,
-    in x and the bias."""
+    in x and the bias, backward or forward (``torch.autograd.forward_ad``); not under ``torch.func`` or a trace."""
     if x is None or weight is None:
         raise ArgumentError("x and weight must not be null")
     if not isinstance(weight, Int4Weight):
         raise ArgumentError(f"weight must be an Int4Weight (got {type(weight).__name__})")
+    _refuse_unseen("int4_linear", x, bias)
     _dtype(x, "x")
     rows, cols = weight.shape
     if x.dim() == 0 or x.shape[-1] != cols:
@@ -248,6 +275,16 @@ def int4_linear(x: torch.Tensor, weight: Int4Weight, bias: torch.Tensor | None =
             raise ArgumentError(f"bias must be {x.dtype} on {x.device} (got {bias.dtype} on {bias.device})")
         if bias.stride(0) != 1:
             bias = bias.contiguous()
+    if forward_ad._current_level >= 0:
+        (x, dx), (bias, db) = forward_ad.unpack_dual(x), (None, None) if bias is None else forward_ad.unpack_dual(bias)
+        if dx is not None or db is not None:
+            y = _linear(x, weight, bias)
+            dy = db.expand_as(y).contiguous() if dx is None else _linear(dx, weight, None if db is None else db.contiguous())
+            return forward_ad.make_dual(y, dy)
+    return _linear(x, weight, bias)
+
+
+def _linear(x, weight, bias):
     if torch.is_grad_enabled() and (x.requires_grad or (bias is not None and bias.requires_grad)):
         return _Int4LinearFn.apply(x, weight, bias)
     return weight._product(x, bias, False)
@@ -292,13 +329,15 @@ def embedding(ids: torch.Tensor, table, scale: float = 1.0, padding_idx: int | N
     bfloat16) for a packed one.
 
     Differentiable in a dense table: row v gets scale times the sum of dy over its tokens, added in token
-    order in fp32 (the same bits every time), the row ``padding_idx`` zeros.  An id outside the table gives
+    order in fp32 (the same bits every time), the row ``padding_idx`` zeros; once, or forward
+    (``torch.autograd.forward_ad``); not under ``torch.func`` or a trace.  An id outside the table gives
     a row of zeros and no gradient, and the device's next ``llmc_sync`` raises ArgumentOutOfRangeError."""
     if ids is None or table is None:
         raise ArgumentError("ids and table must not be null")
     if ids.dtype not in (torch.int64, torch.int32):
         raise ArgumentError(f"ids must be int64 or int32 (got {ids.dtype})")
     packed = isinstance(table, Int4Weight)
+    _refuse_unseen("embedding", ids, table)
     if not packed:
         if table.dim() != 2:
             raise ShapeError(f"table must be [vocab, hidden] (got {list(table.shape)})")
@@ -327,7 +366,15 @@ def embedding(ids: torch.Tensor, table, scale: float = 1.0, padding_idx: int | N
         _lib.call("llmc_int4_embedding", table._ctx, _lib.stream(table._index), ids.data_ptr(), int(ids.dtype == torch.int64),
                   ids.numel(), table._ref, _DTYPES[dtype], scale, out.data_ptr(), hidden)
         return out
-    table = _rows(table, hidden)
+    if forward_ad._current_level >= 0:
+        table, tangent = forward_ad.unpack_dual(table)
+        if tangent is not None:
+            return forward_ad.make_dual(_dense_embedding(ids, table, scale, padding), _dense_embedding(ids, tangent, scale, padding))
+    return _dense_embedding(ids, table, scale, padding)
+
+
+def _dense_embedding(ids, table, scale, padding):
+    table = _rows(table, table.shape[1])
     if torch.is_grad_enabled() and table.requires_grad:
         return _EmbeddingFn.apply(table, ids, scale, padding)
     return _lookup(ids, table, scale)

@@ -1,0 +1,110 @@
+"""The packed products and the embedding under torch's forward mode, its function transforms and its traces: a derivative
+is given or the call is refused, never dropped."""
+
+import pytest
+import torch
+import torch.autograd.forward_ad as forward_ad
+
+from test_packed import ROOT_DEV, check_product, entry, weight
+
+
+def stand_in(monkeypatch, w):
+    """An Int4Weight of a dense matrix on the CPU: what is tested is what surrounds the product."""
+    from llmcompressorsharp_b200 import Int4Weight
+
+    p = object.__new__(Int4Weight)
+    p.shape, p.device = tuple(w.shape), torch.device("cpu")
+
+    def product(self, x, bias, back):  # of values alone, as a kernel's
+        x, bias = torch.tensor(x.tolist()), None if bias is None else torch.tensor(bias.tolist())
+        return x @ w if back else torch.nn.functional.linear(x, w, bias)
+
+    monkeypatch.setattr(Int4Weight, "_product", product)
+    return p
+
+
+@pytest.fixture
+def case(monkeypatch):
+    g = torch.Generator().manual_seed(0)
+    w = torch.randn(5, 7, generator=g)
+    return stand_in(monkeypatch, w), w, torch.randn(3, 7, generator=g), torch.randn(5, generator=g), g
+
+
+def test_tangents_of_a_product(case):
+    """y = x W^T + b is linear: its tangent is dx W^T + db, of either alone too."""
+    from llmcompressorsharp_b200 import int4_linear
+
+    p, w, x, b, g = case
+    dx, db = torch.randn(3, 7, generator=g), torch.randn(5, generator=g)
+    with forward_ad.dual_level():
+        for xs, bs, want in ((forward_ad.make_dual(x, dx), forward_ad.make_dual(b, db), dx @ w.t() + db),
+                             (forward_ad.make_dual(x, dx), b, dx @ w.t()), (x, forward_ad.make_dual(b, db), db.expand(3, 5)),
+                             (forward_ad.make_dual(x, dx), None, dx @ w.t())):
+            y, dy = forward_ad.unpack_dual(int4_linear(xs, p, bs))
+            assert torch.equal(y, torch.nn.functional.linear(x, w, None if bs is None else b))
+            assert torch.allclose(dy, want, rtol=2 ** -20, atol=2 ** -20)
+        assert forward_ad.unpack_dual(int4_linear(x, p, b)).tangent is None
+
+
+def test_a_tangent_keeps_its_gradients(case):
+    """Forward over reverse: y and its tangent both take gradients, dx's through W."""
+    from llmcompressorsharp_b200 import int4_linear
+
+    p, w, x, _, g = case
+    x, dx = x.requires_grad_(True), torch.randn(3, 7, generator=g).requires_grad_(True)
+    with forward_ad.dual_level():
+        y, dy = forward_ad.unpack_dual(int4_linear(forward_ad.make_dual(x, dx), p))
+        gx, gd = torch.autograd.grad((y + 2 * dy).sum(), [x, dx])
+    assert torch.allclose(gx, w.sum(0).expand(3, 7)) and torch.allclose(gd, 2 * w.sum(0).expand(3, 7))
+
+
+def test_transforms_and_traces_are_refused(case):
+    from torch._subclasses import FakeTensorMode
+    from torch.fx.experimental.proxy_tensor import make_fx
+
+    from llmcompressorsharp_b200 import embedding, int4_linear
+    from llmcompressorsharp_b200.errors import NotSupportedError
+
+    p, _, x, b, _ = case
+    ids, table = torch.tensor([0, 2]), torch.randn(4, 6)
+    mode = FakeTensorMode()
+    for f, t in ((lambda t: int4_linear(t, p), x), (lambda t: int4_linear(x, p, t), b), (lambda t: embedding(ids, t), table)):
+        for call in (lambda: torch.func.grad(lambda t: f(t).sum())(t), lambda: torch.func.jvp(f, (t,), (t,)),
+                     lambda: torch.jit.trace(f, (t,), check_trace=False), lambda: make_fx(f)(t), lambda: f(mode.from_tensor(t))):
+            with pytest.raises(NotSupportedError):
+                call()
+    with pytest.raises(NotSupportedError):
+        torch.func.vmap(lambda t: int4_linear(t, p))(torch.stack([x, x]))
+    with pytest.raises(NotSupportedError):
+        torch.func.vmap(lambda i: embedding(i, table))(torch.stack([ids, ids]))
+
+
+def test_what_a_transform_does_not_touch_still_runs(case):
+    """A product of tensors that are not the transform's own."""
+    from llmcompressorsharp_b200 import int4_linear
+
+    p, w, x, b, _ = case
+    with torch.no_grad():
+        assert torch.func.vmap(lambda t: t + 1, randomness="error")(int4_linear(x, p, b)).shape == (3, 5)
+        assert torch.equal(int4_linear(x, p, b), torch.nn.functional.linear(x, w, b))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("tokens", [3, 300])
+def test_tangents_on_the_device(tokens, dtype):
+    from llmcompressorsharp_b200 import embedding, int4_linear
+
+    e, w = entry(70, 130, group=64, device=ROOT_DEV)
+    p = weight(e, 130)
+    g = torch.Generator().manual_seed(1)
+    x, dx = (torch.randn(tokens, 130, generator=g).to(dtype).to(ROOT_DEV) for _ in range(2))
+    b, db = (torch.randn(70, generator=g).to(dtype).to(ROOT_DEV) for _ in range(2))
+    table, dt = (torch.randn(9, 16, generator=g).to(dtype).to(ROOT_DEV) for _ in range(2))
+    ids = torch.randint(0, 9, (tokens,), generator=g).to(ROOT_DEV)
+    with forward_ad.dual_level():
+        y, dy = forward_ad.unpack_dual(int4_linear(forward_ad.make_dual(x, dx), p, forward_ad.make_dual(b, db)))
+        h, dh = forward_ad.unpack_dual(embedding(ids, forward_ad.make_dual(table, dt), 2.0))
+    assert torch.equal(y, int4_linear(x, p, b))
+    check_product(dy, dx.double().cpu(), w, db.double().cpu(), rounded=True)
+    assert torch.equal(h, (table * 2)[ids]) and torch.equal(dh, (dt * 2)[ids])
