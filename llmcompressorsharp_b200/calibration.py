@@ -9,8 +9,8 @@ This module supplies that caller:
 - ``LlamaShape`` presets for the model shapes the job is quoted on;
 - ``LlamaForCalibration``, a random-initialised LLaMA decoder with the usual module names
   (``model.layers.{i}.self_attn.q_proj`` ...), weights ~N(0, 0.02) from a seed, whose
-  forward is ordinary torch (cuBLAS GEMMs and SDPA; on a CUDA device the embedding is the
-  library's): it only produces the activations that reach the hooked Linear layers;
+  forward is ordinary torch (cuBLAS GEMMs, SDPA and torch's embedding, which asserts on an id
+  outside the table): it only produces the activations that reach the hooked Linear layers;
   ``load_compressed`` puts the packed weights a session leaves into it, to run the compressed
   model on the same batches;
 - ``drive(model, batches)``, which runs the forward on each calibration batch and then hands
@@ -29,7 +29,7 @@ from dataclasses import dataclass
 import torch
 import torch.nn.functional as F
 
-from .packed import TokenEmbedding, load_compressed
+from .packed import TokenEmbedding, load_compressed  # noqa: F401 (TokenEmbedding: an embedding to train in its place)
 
 
 @dataclass(frozen=True)
@@ -136,7 +136,7 @@ def _rope(x, cos, sin):
 class _Body(torch.nn.Module):
     def __init__(self, s: LlamaShape, dtype, device, g):
         super().__init__()
-        self.embed_tokens = TokenEmbedding(s.vocab, s.hidden, dtype=dtype, device=device)
+        self.embed_tokens = torch.nn.Embedding(s.vocab, s.hidden, dtype=dtype, device=device)
         with torch.no_grad():
             self.embed_tokens.weight.copy_((torch.randn(s.vocab, s.hidden, generator=g) * 0.02).to(dtype))
         self.embed_tokens.weight.requires_grad_(False)

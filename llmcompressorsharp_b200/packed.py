@@ -414,13 +414,19 @@ class Int4Embedding(torch.nn.Module):
 
 
 class TokenEmbedding(torch.nn.Embedding):
-    """``torch.nn.Embedding`` whose lookup, on a CUDA device, is the library's (the same values).  Types and options
-    that it does not take, and other devices, are torch's."""
+    """``torch.nn.Embedding`` whose lookup, on a CUDA device, is the library's (the same values; a gradient with the same
+    bits every time).  Types and options that it does not take, other devices, and what torch transforms or records
+    (forward mode, ``torch.func``, tracing, compiling, dispatch modes, subclasses of Tensor) are torch's.  Two things differ from torch's on a
+    device: it is differentiable once, and an id outside the table is no device assertion but a row of zeros, which the
+    device's next ``llmc_sync`` reports."""
 
     def forward(self, ids):
         w = self.weight
-        if (w.is_cuda and w.dtype in _DTYPES and ids.dtype in (torch.int64, torch.int32)
-                and self.max_norm is None and not self.scale_grad_by_freq and not self.sparse):
+        if (w.is_cuda and w.dtype in _DTYPES and ids.dtype in (torch.int64, torch.int32) and type(ids) is torch.Tensor
+                and type(w) in (torch.Tensor, torch.nn.Parameter)
+                and self.max_norm is None and not self.scale_grad_by_freq and not self.sparse
+                and forward_ad._current_level < 0 and not torch.compiler.is_compiling() and not torch._C._is_tracing()
+                and torch._C._functorch.peek_interpreter_stack() is None and not torch._C._len_torch_dispatch_stack()):
             return embedding(ids, w, padding_idx=self.padding_idx)
         return super().forward(ids)
 

@@ -108,3 +108,40 @@ def test_tangents_on_the_device(tokens, dtype):
     assert torch.equal(y, int4_linear(x, p, b))
     check_product(dy, dx.double().cpu(), w, db.double().cpu(), rounded=True)
     assert torch.equal(h, (table * 2)[ids]) and torch.equal(dh, (dt * 2)[ids])
+
+
+def test_the_calibration_model_asserts_on_ids_outside_its_table():
+    """The model's embedding is torch's own, whose check of ids ends a session that calibrates on wrong ones: an
+    error on the CPU, an assertion on a device."""
+    from llmcompressorsharp_b200 import CompressionSession, CompressionState, RtnConfig, RtnModifier, SessionStatus
+    from llmcompressorsharp_b200.calibration import LlamaForCalibration, LlamaShape, drive
+
+    m = LlamaForCalibration(LlamaShape(hidden=32, intermediate=48, heads=2, kv_heads=2, layers=1, vocab=11), dtype=torch.float32)
+    assert type(m.model.embed_tokens) is torch.nn.Embedding
+    session = CompressionSession([RtnModifier(RtnConfig(4, True, "channel"))])
+    state = CompressionState(m.linear_weights())
+    assert session.run(state, drive(m, [torch.tensor([[1, 11]])])) == SessionStatus.FAILED and isinstance(session.failure, IndexError)
+
+
+@pytest.mark.gpu
+def test_token_embedding_leaves_to_torch_what_torch_transforms():
+    """Values, tangents, gradients and graphs of an embedding that torch transforms or records are torch's."""
+    from torch.fx.experimental.proxy_tensor import make_fx
+    from torch.func import functional_call, grad, jvp, vmap
+
+    from llmcompressorsharp_b200 import TokenEmbedding
+
+    g = torch.Generator().manual_seed(0)
+    ours, theirs = TokenEmbedding(11, 24, device=ROOT_DEV), torch.nn.Embedding(11, 24, device=ROOT_DEV)
+    theirs.load_state_dict(ours.state_dict())
+    ids, other = (torch.randint(0, 11, (4, 10), generator=g).to(ROOT_DEV) for _ in range(2))
+    dw = torch.randn(11, 24, generator=g).to(ROOT_DEV)
+    got = []
+    for m in (ours, theirs):
+        w = m.weight.detach()
+        f = lambda w: functional_call(m, {"weight": w}, (ids,))  # noqa: B023, E731
+        with forward_ad.dual_level():
+            dual = forward_ad.unpack_dual(functional_call(m, {"weight": forward_ad.make_dual(w, dw)}, (ids,))).tangent
+        got.append([dual, grad(lambda w: f(w).pow(2).sum())(w), *jvp(f, (w,), (dw,)), vmap(m)(ids),
+                    torch.jit.trace(m, (ids,), check_trace=False)(other), make_fx(m)(ids)(other), torch.compile(m, backend="eager")(ids)])
+    assert all(torch.equal(a, b) for a, b in zip(*got))
