@@ -33,6 +33,17 @@
 // tokens the eight warps that dequantise bound it: 29 us for 4096 -> 14336, where the codes alone are read in 5.  Numbers
 // made before the wait for a free stage instead of behind it: no faster.
 // Every wait is bounded.
+//
+// What orders the rings, each turn of a slot by one phase of its barriers:
+//   activations  afull: the copies' bytes complete the phase that the MMA warp waits for; empty: the MMAs that read the
+//                stage complete before the commit's arrival, which the copying thread waits for.
+//   weights      bfull: each dequantising lane fences its stores for the async proxy, the warp syncs, one lane arrives;
+//                a pair's arrival at the leader's barrier stands for shared memory that the arriving SM's half of the
+//                MMA reads.  empty: as above, waited for before the stores.
+//   codes        cfull: the copy's bytes; cempty: all eight warps arrive, the two groups alike, those that read after the
+//                stores made of what they read.  A slot has no new phase before all have seen the last one.
+//   accumulators tfull: the commit after a fold's last MMA; tempty: each epilogue warp's loads are waited for in the
+//                statement that makes them, and fenced, before its arrival.
 #include "int4.cuh"
 #include "ops.h"
 #include "tc_common.cuh"
@@ -104,6 +115,26 @@ __device__ __forceinline__ void combo(int c, int& xp, int& wp) {
 // rows of different parity, so that its 16-byte loads (rows 64 bytes apart) touch every bank once, and of
 // different bit 2, so that its stores into the 128-byte swizzle do.
 __device__ __forceinline__ int row_of(int lane) { return (0x36271450 >> (lane / 4 * 4)) & 7; }
+
+// Reads of a tile of codes, which a bulk copy fills again once it is let go of.  Volatile: an ordinary load may be done
+// later, or again, instead of keeping its value, and the fp32 kernels are short of registers.  With ordinary loads and the
+// tile let go of right after them, fp32 gradients on two streams at once (32 of 80) had codes of a later tile in them; with
+// these and the same order none of 48,000 products of any type did.
+__device__ __forceinline__ uint4 read_codes(uint32_t addr) {
+    uint4 v;
+    asm volatile("ld.volatile.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr) : "memory");
+    return v;
+}
+__device__ __forceinline__ float read_scale(uint32_t addr) {
+    float v;
+    asm volatile("ld.volatile.shared.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+    return v;
+}
+__device__ __forceinline__ uint32_t read_zero(uint32_t addr) {
+    uint32_t v;
+    asm volatile("ld.volatile.shared.u8 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
+    return v;
+}
 
 // A scale and zero ready for eight weights at a time.
 template <typename T, int PIECES> struct Scale {
@@ -451,19 +482,18 @@ __global__ void __launch_bounds__(32 * (3 + (PIECES == 3 ? 8 : 4) + DQ_WARPS), 1
                     if (lane == 0) mbar_arrive(&cempty[cs]);
                     return true;
                 }
-                const unsigned char* tile = codes + cs * CODE_BYTES;
+                const uint32_t tile = smem_u32(codes) + cs * CODE_BYTES;
                 uint4 q[4];
                 Scale<T, PIECES> sc[4][GROUPS];
 #pragma unroll
                 for (int i = 0; i < 4; i++) {
-                    const unsigned char* rec = tile + (2 * w + i / 2) * a.v.rec;
+                    const uint32_t rec = tile + (2 * w + i / 2) * a.v.rec;
                     const int in = 8 * (i & 1) + r8;
-                    q[i] = *reinterpret_cast<const uint4*>(rec + in * 64 + t * 16);
-                    const float* scales = reinterpret_cast<const float*>(rec + 1024) + in * ng;
-                    const unsigned char* zeros = rec + 1024 + 64 * ng + in * ng;
+                    q[i] = read_codes(rec + in * 64 + t * 16);
+                    const uint32_t scales = rec + 1024 + 4 * in * ng, zeros = rec + 1024 + 64 * ng + in * ng;
 #pragma unroll
                     for (int c = 0; c < GROUPS; c++)
-                        sc[i][c].set(scales[slot_of(c, ng)] * e[DIR == 0 ? i : c], zeros[slot_of(c, ng)]);
+                        sc[i][c].set(read_scale(scales + 4 * slot_of(c, ng)) * e[DIR == 0 ? i : c], read_zero(zeros + slot_of(c, ng)));
                 }
                 if (!mbar_wait(&empty[sg], ph ^ 1u, abort_flag, a.err, a.wait_limit)) return false;
                 unsigned char* b = smem + sg * STAGE_BYTES + A_BYTES;
@@ -485,9 +515,8 @@ __global__ void __launch_bounds__(32 * (3 + (PIECES == 3 ? 8 : 4) + DQ_WARPS), 1
                 if (lane == 0) {
                     if constexpr (CG == 2) mbar_arrive_cluster_cta(mapa_shared(smem_u32(&bfull[sg]), 0));
                     else mbar_arrive(&bfull[sg]);
-                    // The tile of codes is let go of only now, when what was read of it has gone into the stores above: let
-                    // go of right after the loads, it was refilled too early at times beside another stream's product
-                    // (fp32 gradients, some of 1,256 tiles in most runs).
+                    // The tile of codes is let go of when what was read of it has gone into the stores above, so that its
+                    // reads come first by their data, too (no slower than right after them).
                     mbar_arrive(&cempty[cs]);
                 }
                 return true;
