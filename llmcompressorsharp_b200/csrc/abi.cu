@@ -90,20 +90,18 @@ llmc_status injected_fault(const char* fn) {
     return LLMC_OK;
 }
 
-// Synchronises the stream and reports the device error words, clearing them: word 2, a bounded
-// device wait that gave up (written by the tensor-core kernels), as LLMC_ERR_TIMEOUT; word 3, a
-// Hessian that was not positive definite in a factorisation run with deferred errors, as
-// LLMC_ERR_NOT_PD; and for llmc_sync (ids) word 4, an embedding id outside its table, as
-// LLMC_ERR_OUT_OF_RANGE.
+// Synchronises the stream and reports the device error words: word 2, a bounded device wait that
+// gave up (written by the tensor-core kernels), as LLMC_ERR_TIMEOUT; word 3, a Hessian that was not
+// positive definite in a factorisation run with deferred errors, as LLMC_ERR_NOT_PD; and for
+// llmc_sync (ids) word 4, an embedding id outside its table, as LLMC_ERR_OUT_OF_RANGE.  The word that
+// is reported is cleared (a wait that gave up takes word 3 with it: what was factored after it means
+// nothing); the others stay for the next call.
 llmc_status device_error_check(llmc_ctx* ctx, bool ids) {
-    const int words = ids ? 3 : 2;
-    LLMC_CUDA_TRY(cudaMemcpyAsync(ctx->hflags + 2, ctx->dflags + 2, words * sizeof(int), cudaMemcpyDeviceToHost, ctx->stream));
+    LLMC_CUDA_TRY(cudaMemcpyAsync(ctx->hflags + 2, ctx->dflags + 2, 3 * sizeof(int), cudaMemcpyDeviceToHost, ctx->stream));
     LLMC_CUDA_TRY(cudaStreamSynchronize(ctx->stream));
     const int timeout = ctx->hflags[2], not_pd = ctx->hflags[3], bad_id = ids ? ctx->hflags[4] : 0;
-    if (timeout || not_pd || bad_id) {
-        ctx->hflags[2] = ctx->hflags[3] = ctx->hflags[4] = 0;
-        LLMC_CUDA_TRY(cudaMemsetAsync(ctx->dflags + 2, 0, words * sizeof(int), ctx->stream));
-    }
+    const int first = timeout ? 2 : not_pd ? 3 : 4, words = timeout ? 2 : not_pd || bad_id ? 1 : 0;
+    if (words) LLMC_CUDA_TRY(cudaMemsetAsync(ctx->dflags + first, 0, words * sizeof(int), ctx->stream));
     if (timeout)
         return fail(LLMC_ERR_TIMEOUT, "a bounded wait inside a tensor-core kernel gave up; results of the "
                     "affected calls are incomplete");

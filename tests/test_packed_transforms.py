@@ -145,3 +145,18 @@ def test_token_embedding_leaves_to_torch_what_torch_transforms():
         got.append([dual, grad(lambda w: f(w).pow(2).sum())(w), *jvp(f, (w,), (dw,)), vmap(m)(ids),
                     torch.jit.trace(m, (ids,), check_trace=False)(other), make_fx(m)(ids)(other), torch.compile(m, backend="eager")(ids)])
     assert all(torch.equal(a, b) for a, b in zip(*got))
+
+
+@pytest.mark.gpu
+def test_compiled_callers_run_the_kernels():
+    """torch.compile breaks its graph at the calls and runs them as they are."""
+    from llmcompressorsharp_b200 import embedding, int4_linear
+
+    p = weight(entry(64, 128, group=64, device=ROOT_DEV)[0], 128)
+    x, table = torch.randn(4, 128, device=ROOT_DEV), torch.randn(40, 16, device=ROOT_DEV)
+    ids = torch.randint(0, 40, (7,), device=ROOT_DEV)
+    assert torch.equal(torch.compile(lambda x: int4_linear(x * 2, p) + 1, backend="eager")(x), int4_linear(x * 2, p) + 1)
+    assert torch.equal(torch.compile(lambda i: embedding(i, table, 2.0) + 1, backend="eager")(ids), embedding(ids, table, 2.0) + 1)
+    xs = x.clone().requires_grad_(True)
+    (dx,) = torch.autograd.grad(torch.compile(lambda x: int4_linear(x * 2, p).sum(), backend="eager")(xs), xs)
+    assert torch.equal(dx, torch.autograd.grad(int4_linear(xs * 2, p).sum(), xs)[0])
