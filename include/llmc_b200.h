@@ -111,7 +111,12 @@ llmc_status llmc_set_wait_limit(llmc_ctx* ctx, int64_t tries);
  * errors off.  on = 0 (the default) restores the synchronous reporting.  No reference counterpart: it lets one host thread
  * enqueue a layer's solve while other streams keep running. */
 llmc_status llmc_set_deferred_errors(llmc_ctx* ctx, int32_t on);
+/* Waits for the context's stream and reports the first pending device error: LLMC_ERR_TIMEOUT, then LLMC_ERR_NOT_PD,
+ * then LLMC_ERR_OUT_OF_RANGE (an embedding id outside its table).  What it reports is cleared, the others stay pending. */
 llmc_status llmc_sync(llmc_ctx* ctx);
+/* The same for the first two, for the end of a solve: an embedding id stays pending, since the lookup that it
+ * belongs to may be anyone's. */
+llmc_status llmc_wait(llmc_ctx* ctx);
 /* Number of kernels this context has launched since creation (diagnostics / bench). */
 llmc_status llmc_launch_count(llmc_ctx* ctx, int64_t* out);
 

@@ -67,6 +67,7 @@ _SIGS = {
     "llmc_set_wait_limit": [P, I64],
     "llmc_set_deferred_errors": [P, I32],
     "llmc_sync": [P],
+    "llmc_wait": [P],
     "llmc_launch_count": [P, C.POINTER(I64)],
     "llmc_hessian_create": [P, I64, C.POINTER(P)],
     "llmc_hessian_update": [P, P, I32, I64, I64],

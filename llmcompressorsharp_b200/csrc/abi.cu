@@ -288,6 +288,12 @@ llmc_status llmc_sync(llmc_ctx* ctx) {
     return device_error_check(ctx, true);
 }
 
+llmc_status llmc_wait(llmc_ctx* ctx) {
+    LLMC_ENTRY();
+    CTX_CHECK(ctx);
+    return device_error_check(ctx);
+}
+
 llmc_status llmc_launch_count(llmc_ctx* ctx, int64_t* out) {
     LLMC_ENTRY();
     NULL_CHECK(ctx, "ctx");

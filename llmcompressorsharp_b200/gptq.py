@@ -248,7 +248,7 @@ class GPTQModifier(ModifierBase):
         alias = self._alias
         # Factor every distinct Hessian first, with the device context's errors deferred: the
         # factorisations are enqueued back to back (none reads a flag back to the host), and one
-        # llmc_sync per device then reports whether any Hessian had no Cholesky factor.  Those
+        # llmc_wait per device then reports whether any Hessian had no Cholesky factor.  Those
         # devices factor their Hessians again synchronously, which takes the reference's
         # pseudo-inverse fallback (HessianInverseSolver.cs:85-91); every weight is replaced only
         # after all factors exist.
@@ -268,7 +268,7 @@ class GPTQModifier(ModifierBase):
                 with torch.cuda.device(dev):
                     for key, src in items:
                         ucache[key] = HessianInverseSolver.upper(src.raw(), self.config.dampening_frac, upper_only=True)
-                _lib.call("llmc_sync", c)
+                _lib.call("llmc_wait", c)
             except NotPositiveDefiniteError:
                 redo = True
             finally:

@@ -392,7 +392,7 @@ class _Overlap:
         self.solve_sms = max(1, int(reserve_sms))
         _lib.call("llmc_set_sm_limit", C.c_void_p(self.cs), C.c_int32(self.solve_sms))
         # The factorisation decides a non-PD Hessian on the device, so enqueueing a solve never
-        # waits for the GPU; a failure surfaces at the llmc_sync that ends the job.
+        # waits for the GPU; a failure surfaces at the llmc_wait that ends the job.
         _lib.call("llmc_set_deferred_errors", C.c_void_p(self.cs), C.c_int32(1))
         # One stream, context and scratch set per site for ``run``: a layer's sites are
         # independent given their Hessians, so their solves (chains of mostly small, dependent
@@ -605,7 +605,7 @@ class _Overlap:
         """Waits for the solve stream and raises the first deferred device error (a Hessian
         that was not positive definite, a bounded wait that gave up) of either context."""
         for c in self.solve_contexts() + [self.ch]:
-            _lib.call("llmc_sync", C.c_void_p(c))
+            _lib.call("llmc_wait", C.c_void_p(c))
 
     # ---- one process per GPU ------------------------------------------------------------------
     DIST_SETS = 6  # Hessian handle sets in flight per rank

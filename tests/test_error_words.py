@@ -47,3 +47,33 @@ def test_a_bad_id_outlives_the_error_that_is_reported_before_it(ctx):
         assert [lib.llmc_sync(c) for _ in range(3)] == [NOT_PD, OUT_OF_RANGE, OK]
     bad_id(lib, c)
     assert [lib.llmc_sync(c) for _ in range(2)] == [OUT_OF_RANGE, OK]
+
+
+def test_a_solve_leaves_an_id_of_another_lookup_pending(ctx):
+    lib, c = ctx
+    bad_id(lib, c)
+    assert lib.llmc_wait(c) == OK
+    not_pd(lib, c)
+    assert [lib.llmc_wait(c), lib.llmc_wait(c), lib.llmc_sync(c), lib.llmc_sync(c)] == [NOT_PD, OK, OUT_OF_RANGE, OK]
+
+
+def test_a_gptq_session_is_not_failed_by_an_id_of_another_lookup():
+    from llmcompressorsharp_b200 import CompressionSession, CompressionState, GPTQConfig, GPTQModifier, SessionStatus, _lib, embedding
+    from llmcompressorsharp_b200.errors import ArgumentOutOfRangeError
+
+    embedding(torch.tensor([3], device=ROOT_DEV), torch.ones(3, 8, device=ROOT_DEV))
+    lin = torch.nn.Linear(64, 32, bias=False, device=ROOT_DEV)
+    state = CompressionState({"lin.weight": lin.weight.detach()})
+    state.named_modules = {"lin": lin}
+
+    def batches():
+        for i in range(2):
+            x = torch.randn(96, 64, generator=torch.Generator().manual_seed(i)).to(ROOT_DEV)
+            lin(x)
+            yield x
+
+    session = CompressionSession([GPTQModifier(GPTQConfig(num_bits=4, symmetric=True, strategy="channel"))])
+    assert session.run(state, batches()) == SessionStatus.COMPLETED, session.failure
+    assert "lin.weight" in state.compressed
+    with pytest.raises(ArgumentOutOfRangeError):
+        _lib.call("llmc_sync", _lib.ctx_for(0))
