@@ -393,7 +393,11 @@ class Int4Linear(torch.nn.Module):
             self.register_buffer("bias", bias)
 
     def forward(self, x):
-        return int4_linear(x, self.packed_weight, self.bias)
+        bias = self.bias
+        if torch.is_autocast_enabled("cuda") and x.is_cuda and x.dtype in _DTYPES:  # as torch.nn.Linear is cast
+            dtype = torch.get_autocast_dtype("cuda")
+            x, bias = x.to(dtype), None if bias is None else bias.to(dtype)
+        return int4_linear(x, self.packed_weight, bias)
 
     def extra_repr(self):
         w = self.packed_weight
