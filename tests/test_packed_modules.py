@@ -28,3 +28,52 @@ def test_autocast_casts_what_torch_casts(dtype):
         check_product(y.detach(), xs.detach().to(dtype).double().cpu(), w, m.bias.detach().to(dtype).double().cpu(), rounded=True)
     with torch.autocast("cuda", dtype, enabled=False):
         assert m(x).dtype == torch.float32
+
+
+@pytest.fixture
+def made(monkeypatch):
+    """load_compressed on the CPU: the packed weights are stand-ins that know their shape."""
+    from llmcompressorsharp_b200 import Int4Weight
+
+    def from_entry(e, cols):
+        p = object.__new__(Int4Weight)
+        p.shape, p.strategy, p.group_size = (e["rows"], cols), "channel", cols
+        return p
+
+    monkeypatch.setattr(Int4Weight, "from_entry", staticmethod(from_entry))
+    return lambda m: {f"{n}.weight": {"codes": 1, "num_bits": 4, "rows": m.get_submodule(n).weight.shape[0]} for n in ("a", "b", "c", "d")}
+
+
+def test_hooks_and_training_go_with_the_module(made):
+    from llmcompressorsharp_b200 import Int4Embedding, Int4Linear, load_compressed
+
+    m = torch.nn.ModuleDict({"a": torch.nn.Linear(8, 4), "b": torch.nn.Embedding(5, 8), "c": torch.nn.Linear(8, 4), "d": torch.nn.Linear(8, 4)})
+    m["a"].eval()
+    seen = []
+    handles = [m["a"].register_forward_hook(lambda mod, args, kwargs, out: seen.append(("a", kwargs)), with_kwargs=True),
+               m["a"].register_forward_pre_hook(lambda mod, args: seen.append("pre")),
+               m["a"].register_full_backward_hook(lambda mod, gi, go: seen.append("back")),
+               m["b"].register_forward_hook(lambda mod, args, out: out + 1)]
+    assert load_compressed(m, made(m)) == ["a", "b", "c", "d"]
+    assert type(m["a"]) is Int4Linear and type(m["b"]) is Int4Embedding
+    assert not m["a"].training and m["b"].training and m["c"].training
+    m["a"].forward = lambda x: x * 2
+    m["b"].forward = lambda ids: ids * 2
+    x = torch.ones(2, 8, requires_grad=True)
+    m["a"](x).sum().backward()
+    assert seen == ["pre", ("a", {}), "back"]
+    assert torch.equal(m["b"](torch.tensor([1, 2])), torch.tensor([3, 5]))
+    for h in handles:
+        h.remove()
+    m["a"](x)
+    assert len(seen) == 3 and torch.equal(m["b"](torch.tensor([1, 2])), torch.tensor([2, 4]))
+
+
+def test_what_a_packed_module_cannot_hold_stays_dense(made):
+    """A type that the products do not take, and a weight that a hook computes before each call."""
+    from llmcompressorsharp_b200 import load_compressed
+
+    m = torch.nn.ModuleDict({"a": torch.nn.Linear(8, 4).double(), "b": torch.nn.Embedding(5, 8, dtype=torch.float64),
+                             "c": torch.nn.utils.spectral_norm(torch.nn.Linear(8, 4)), "d": torch.nn.Linear(8, 4)})
+    assert load_compressed(m, made(m)) == ["d"]
+    assert m["a"](torch.ones(2, 8, dtype=torch.float64)).dtype == torch.float64 and m["c"](torch.ones(2, 8)).shape == (2, 4)
