@@ -37,6 +37,9 @@ llmc_status check_sizes(int64_t rows, int64_t cols, int64_t gs) {
     if (rows > MAX_DIM || cols > MAX_DIM) return fail(LLMC_ERR_OUT_OF_RANGE, "a packed weight has at most 2^30 rows and columns");
     if (gs < 16 && gs < cols)
         return fail(LLMC_ERR_UNSUPPORTED, "group_size must be at least 16, or at least the columns (got %lld)", (long long)gs);
+    // the kernels count the layout's columns, up to twice the weight's (groups of 16 take 32 each), in 32 bits
+    if (gs < cols && (cols + gs - 1) / gs * w4::up(gs, 32) > MAX_DIM)
+        return fail(LLMC_ERR_OUT_OF_RANGE, "%lld columns in groups of %lld take more than 2^30 of the layout", (long long)cols, (long long)gs);
     return LLMC_OK;
 }
 

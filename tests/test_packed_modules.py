@@ -77,3 +77,18 @@ def test_what_a_packed_module_cannot_hold_stays_dense(made):
                              "c": torch.nn.utils.spectral_norm(torch.nn.Linear(8, 4)), "d": torch.nn.Linear(8, 4)})
     assert load_compressed(m, made(m)) == ["d"]
     assert m["a"](torch.ones(2, 8, dtype=torch.float64)).dtype == torch.float64 and m["c"](torch.ones(2, 8)).shape == (2, 4)
+
+
+def test_a_layout_of_more_columns_than_32_bits_count_is_refused():
+    """Groups of 16 columns take 32 of the layout: 2^30 columns would be 2^31 there."""
+    import ctypes as C
+
+    from llmcompressorsharp_b200 import _lib
+
+    lib = _lib.load()
+    p, x = C.c_int64(), C.c_int64()
+    assert lib.llmc_int4_layout_sizes(1, 1 << 30, 16, C.byref(p), C.byref(x)) == 10  # LLMC_ERR_OUT_OF_RANGE
+    assert lib.llmc_int4_layout_sizes(1, 1 << 30, 100, C.byref(p), C.byref(x)) == 10
+    assert lib.llmc_int4_layout_sizes(1, 1 << 29, 16, C.byref(p), C.byref(x)) == 0
+    assert lib.llmc_int4_layout_sizes(1, 1 << 30, 128, C.byref(p), C.byref(x)) == 0
+    assert lib.llmc_int4_layout_sizes(1, 1 << 30, 1 << 30, C.byref(p), C.byref(x)) == 0
