@@ -22,7 +22,7 @@ from .sparsegpt import SparseGPTConfig, SparseGPTModifier, sparsegpt_prune_u
 from .awq import AWQConfig, AWQModifier, awq_search, scale_apply
 from .session import (CompressionSession, CompressionState, ModifierBase, ModifierLifecycleError, SessionStatus,
                       TargetMatcher)
-from .packed import Int4Embedding, Int4Linear, Int4Weight, TokenEmbedding, embedding, int4_linear, load_compressed
+from .packed import Int4Embedding, Int4Linear, Int4Weight, TokenEmbedding, check_ids, embedding, int4_linear, load_compressed
 from .output import CompressedTensorsWriter, SafetensorsWriter
 
 __all__ = [n for n in dir() if not n.startswith("_")]

@@ -24,12 +24,14 @@ afterwards from those Hessians).
 
 from __future__ import annotations
 
+import warnings
 from dataclasses import dataclass
 
 import torch
 import torch.nn.functional as F
 
-from .packed import TokenEmbedding, load_compressed  # noqa: F401 (TokenEmbedding: an embedding to train in its place)
+from .errors import ArgumentOutOfRangeError
+from .packed import TokenEmbedding, check_ids, load_compressed  # noqa: F401 (TokenEmbedding: an embedding to train in its place)
 
 
 @dataclass(frozen=True)
@@ -198,7 +200,17 @@ def calibration_batches(vocab: int, sequences: int, seq_len: int, batch: int, se
 
 def drive(model: torch.nn.Module, batches):
     """Run the calibration forward on each batch (firing every hook the modifiers attached),
-    then yield the batch to the session."""
+    then yield the batch to the session.  Where the model's embedding is the library's (a
+    compressed model's), an id outside its table ends the batches with an error, before the
+    session's end; one that an earlier lookup left is a warning."""
+    checked = isinstance(model, torch.nn.Module)
+    try:
+        if checked:
+            check_ids(model)
+    except ArgumentOutOfRangeError as e:
+        warnings.warn(f"before the first batch: {e}", stacklevel=2)
     for b in batches:
         model(b)
         yield b
+    if checked:
+        check_ids(model)

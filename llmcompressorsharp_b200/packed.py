@@ -435,6 +435,19 @@ class TokenEmbedding(torch.nn.Embedding):
         return super().forward(ids)
 
 
+def check_ids(model: torch.nn.Module) -> None:
+    """Waits for the devices of the library's embeddings in ``model`` and raises ArgumentOutOfRangeError if a lookup on one
+    of them, since the last check, had an id outside its table (its row was zeros).  Other pending errors of the device
+    are raised as well."""
+    if model is None:
+        raise ArgumentError("model must not be null")
+    devices = {m.packed_weight.device if isinstance(m, Int4Embedding) else m.weight.device
+               for m in model.modules() if isinstance(m, (Int4Embedding, TokenEmbedding))}
+    for device in devices:
+        if device.type == "cuda":
+            _lib.call("llmc_sync", _lib.ctx_for(device.index))
+
+
 # What a module holds for its caller around its forward pass.  The dicts are shared, so that a hook's handle still
 # takes it out.
 _HOOKS = ("_forward_hooks", "_forward_hooks_with_kwargs", "_forward_hooks_always_called", "_forward_pre_hooks",

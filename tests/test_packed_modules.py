@@ -92,3 +92,27 @@ def test_a_layout_of_more_columns_than_32_bits_count_is_refused():
     assert lib.llmc_int4_layout_sizes(1, 1 << 29, 16, C.byref(p), C.byref(x)) == 0
     assert lib.llmc_int4_layout_sizes(1, 1 << 30, 128, C.byref(p), C.byref(x)) == 0
     assert lib.llmc_int4_layout_sizes(1, 1 << 30, 1 << 30, C.byref(p), C.byref(x)) == 0
+
+
+@pytest.mark.gpu
+def test_a_session_over_a_packed_table_hears_of_a_bad_id():
+    from llmcompressorsharp_b200 import (CompressionSession, CompressionState, Int4Embedding, Int4Weight, RtnConfig, RtnModifier, SessionStatus,
+                                         embedding)
+    from llmcompressorsharp_b200.calibration import drive
+    from llmcompressorsharp_b200.errors import ArgumentOutOfRangeError
+
+    lin = torch.nn.Linear(64, 32, bias=False, device=ROOT_DEV)
+    w = torch.randn(20, 64, generator=torch.Generator().manual_seed(0)).to(ROOT_DEV)
+    m = torch.nn.Sequential(Int4Embedding(Int4Weight.from_float(w, RtnConfig(4, True, "channel")), torch.float32), lin)
+
+    def run(ids):
+        s = CompressionSession([RtnModifier(RtnConfig(4, True, "channel"))])
+        return s.run(CompressionState({"1.weight": lin.weight.detach()}), drive(m, [torch.tensor([i], device=ROOT_DEV) for i in ids])), s.failure
+
+    assert run([3, 19]) == (SessionStatus.COMPLETED, None)
+    status, failure = run([3, 20])
+    assert status == SessionStatus.FAILED and isinstance(failure, ArgumentOutOfRangeError)
+    assert run([3, 19]) == (SessionStatus.COMPLETED, None)
+    embedding(torch.tensor([-1], device=ROOT_DEV), w)  # anyone's
+    with pytest.warns(UserWarning, match="outside its table"):
+        assert run([3, 19]) == (SessionStatus.COMPLETED, None)
