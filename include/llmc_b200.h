@@ -387,8 +387,9 @@ llmc_status llmc_int4_dequantize(llmc_ctx* ctx, void* stream, const llmc_int4_we
                                  int64_t ldo);
 /* y [tokens, ldy] = x [tokens, ldx] W^T + bias (bias [rows], may be NULL), all of dtype.  Sums in fp32,
  * one rounding.  With few tokens (32 and fewer always, up to 256 in many cases) the codes enter as
- * exact integers; with more, and in the gradient, W is rounded to a 16-bit dtype first, or kept to 24
- * bits for F32.  The sums of integers times x come before the scale: they must stay in fp32's range. */
+ * exact integers; with more, and in the gradient, W is rounded to a 16-bit dtype first (F16: a scale below
+ * 2^-13 of the largest of its row, or in the gradient of its group's column, loses bits), and for F32 a product
+ * x W is kept to 2^-22 of itself.  The sums of integers times x come before the scale: they must stay in fp32's range. */
 llmc_status llmc_int4_linear_workspace(llmc_ctx* ctx, const llmc_int4_weight* w, const void* x, int32_t dtype,
                                        int64_t tokens, int64_t ldx, int64_t* bytes);
 llmc_status llmc_int4_linear(llmc_ctx* ctx, void* stream, const llmc_int4_weight* w, const void* x, int32_t dtype,
@@ -411,8 +412,8 @@ llmc_status llmc_embedding(llmc_ctx* ctx, void* stream, const void* ids, int32_t
 /* The same from a packed table, in dtype. */
 llmc_status llmc_int4_embedding(llmc_ctx* ctx, void* stream, const void* ids, int32_t ids64, int64_t tokens,
                                 const llmc_int4_weight* w, int32_t dtype, float scale, void* out, int64_t ldo);
-/* dtable [vocab, hidden] (contiguous, all of it written) = scale * sum of the dy rows of each id, in token
- * order, in fp32, rounded once to dtype: two calls give the same bits.  The row padding_idx (-1: none) gets zeros, ids
+/* dtable [vocab, hidden] (contiguous, all of it written) = scale * sum of the dy rows of each id, in fp32 in a fixed
+ * order (by token; of more than 32, runs of 32 and then their sums), rounded once to dtype: two calls give the same bits.  The row padding_idx (-1: none) gets zeros, ids
  * outside the table no part. */
 llmc_status llmc_embedding_grad_workspace(llmc_ctx* ctx, int64_t tokens, int64_t vocab, int64_t hidden, int64_t* bytes);
 llmc_status llmc_embedding_grad(llmc_ctx* ctx, void* stream, const void* ids, int32_t ids64, int64_t tokens, const void* dy,

@@ -6,8 +6,9 @@
 // caller); the lookup is the first step of that forward, and its gradient completes the straight-through
 // backward of FakeQuantize (FakeQuantizeFunction.cs:56-68) for a quantised table.
 //
-// The gradient adds each row's tokens in token order, whatever ran when: the ids are sorted (stable), every
-// row sums its own run in fp32, and runs of more than RUN tokens are cut into pieces that are joined in order.
+// The gradient adds each row's tokens in a fixed order, whatever ran when: the ids are sorted (stable), every
+// row sums its own run in token order in fp32, and runs of more than RUN tokens are cut into pieces whose sums are
+// added in order, or of more than 64 pieces every sixteenth in order and then those sixteen.
 // No float atomics, so two calls give the same bits.
 #include "ops.h"
 #include "tc_common.cuh"

@@ -168,9 +168,10 @@ __global__ void __launch_bounds__(256) rows_kernel(const View v, const I* ids, i
 
 // ---- x in the layout's columns ------------------------------------------------------------------
 // out[p][t][kv], p < pieces: x[t][k(kv)] in its own 16-bit type, zeros where no column is; or, for fp32,
-// three bf16 pieces whose sum is x exactly: each takes the eight leading bits that are left (truncated, so
-// nothing overflows).  An infinity or a NaN is all in the first piece; a fourth (pieces = 4) is the first with
-// zeros in their place, for products with the smaller pieces of a weight, where an infinity times zero or
+// three bf16 pieces whose sum is x exactly: each takes the eight leading bits that are left, rounded to nearest so
+// that what the products of pieces leave out (k_int4_gemm.cu) is small and of either sign (truncated where the
+// first would round to an infinity).  An infinity or a NaN is all in the first piece; a fourth (pieces = 4) is the
+// first with zeros in their place, for products with the smaller pieces of a weight, where an infinity times zero or
 // times the other sign would make a NaN that the whole product does not have.
 template <typename T>
 __global__ void __launch_bounds__(256) stage_kernel(const T* x, int64_t tokens, int64_t n, int64_t ldx, int64_t pitch,
@@ -188,11 +189,12 @@ __global__ void __launch_bounds__(256) stage_kernel(const T* x, int64_t tokens, 
                 const float f = v;
                 const uint32_t b = __float_as_uint(f);
                 const bool fin = isfinite(f);
-                const float hi = __uint_as_float(b & 0xFFFF0000u);
+                float hi = to_f<__nv_bfloat16>(__float2bfloat16_rn(f));
+                if (!isfinite(hi)) hi = __uint_as_float(b & 0xFFFF0000u);
                 const float r1 = fin ? __fsub_rn(f, hi) : 0.f;
-                const float mid = __uint_as_float(__float_as_uint(r1) & 0xFFFF0000u);
+                const float mid = to_f<__nv_bfloat16>(__float2bfloat16_rn(r1));
                 const float lo = __fsub_rn(r1, mid);
-                p[0].h[j] = f != f ? (uint16_t)0x7FC0 : (uint16_t)(b >> 16);
+                p[0].h[j] = f != f ? (uint16_t)0x7FC0 : (uint16_t)(__float_as_uint(hi) >> 16);
                 p[1].h[j] = (uint16_t)(__float_as_uint(mid) >> 16);
                 p[2].h[j] = (uint16_t)(__float_as_uint(lo) >> 16);
                 p[3].h[j] = fin ? p[0].h[j] : (uint16_t)0;

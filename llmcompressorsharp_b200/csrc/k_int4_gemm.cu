@@ -12,11 +12,16 @@
 // scale goes in as a sum of two 16-bit numbers, fma(v, s_hi, v s_lo), v an exact integer.  That is the weight
 // that the quantisers themselves hand back in a model of that type (FakeQuantizeFunction.cs:39-44 rounds its
 // last product to the tensor's type), and it lets a product run over any group size without leaving TMEM.  In
-// fp16 the scales are first brought near one by a power of two per row (forward) or per group (gradient) that
-// the epilogue takes back in fp32, so small scales keep their bits.
+// fp16 the scales are first brought near one by a power of two per row (forward) or per group over all rows (gradient)
+// that the epilogue takes back in fp32, so scales of any size keep their bits, and ratios do as far as fp16 goes: beside
+// the largest scale s of its row (its group's column) a scale counts to 2^-24 s, so that its weights have 2^-11 down to
+// about 2^-13 s and lose a bit for each power of two below.
 //
-// fp32 activations come as three bf16 pieces that add up to them exactly; W is split the same way after its
-// product in fp32, and the six piece products down to 2^-24 are added, small ones first.  Tensor-core fp32
+// fp32 activations come as three bf16 pieces that add up to them exactly (rounded to nearest, so the second and third
+// are 2^-8 and 2^-17 of the leading power at most); W is split after its product in fp32 by truncation (2^-7, 2^-15).  Six
+// piece products are added, small ones first; the three left out are x1 w2 and x2 w1, 2^-23 and 2^-24, and less, so a
+// term is off by 2^-22.4 of itself at most, with either sign (of 4 million, 2^-22.6; 2^-21.2 and always towards zero with x
+// truncated, too).  Tensor-core fp32
 // accumulation truncates, so TMEM then holds 256 terms of the contraction at most before the epilogue adds them
 // to fp32 registers.
 //

@@ -255,7 +255,9 @@ def int4_linear(x: torch.Tensor, weight: Int4Weight, bias: torch.Tensor | None =
 
     Sums are fp32 and rounded once.  With few rows of x (32 and fewer always, up to 256 in many cases) the
     codes are multiplied as exact integers; with more, and in the backward pass, W is rounded to x's 16-bit
-    type first (as a dequantised weight of that type is), or kept to 24 bits for float32.  Differentiable once,
+    type first (as a dequantised weight of that type is), or for float32 each product is kept to 2^-22 of itself.
+    In float16 a scale below 2^-13 of the largest in its row (in the backward pass: of its group's in any row) loses bits
+    then.  Differentiable once,
     in x and the bias, backward or forward (``torch.autograd.forward_ad``); not under ``torch.func`` or a trace."""
     if x is None or weight is None:
         raise ArgumentError("x and weight must not be null")
@@ -328,8 +330,8 @@ def embedding(ids: torch.Tensor, table, scale: float = 1.0, padding_idx: int | N
     ``Int4Weight``; the result is [..., hidden] of the dense table's type, or of ``dtype`` (default
     bfloat16) for a packed one.
 
-    Differentiable in a dense table: row v gets scale times the sum of dy over its tokens, added in token
-    order in fp32 (the same bits every time), the row ``padding_idx`` zeros; once, or forward
+    Differentiable in a dense table: row v gets scale times the sum of dy over its tokens, added in fp32 in a fixed
+    order (by token; of more than 32, runs of 32 tokens and then their sums; the same bits every time), the row ``padding_idx`` zeros; once, or forward
     (``torch.autograd.forward_ad``); not under ``torch.func`` or a trace.  An id outside the table gives
     a row of zeros and no gradient, and the device's next ``llmc_sync`` raises ArgumentOutOfRangeError."""
     if ids is None or table is None:
