@@ -82,7 +82,7 @@ class Int4Weight:
     ``codes`` are as ``rtn_quantize`` and the GPTQ calls write them for num_bits <= 4:
     (q - zp) & 0xF, two per byte, the even column in the high nibble (Int4PackedTensor.cs:47-69).
     They are laid out anew (and rounded up to 128 rows and columns); the tensors passed in are not
-    kept.  Groups have at least 16 columns.  The weight is constant: its scales take no gradient.  It
+    kept.  Zero-points are in [0, 2^num_bits).  Groups have at least 16 columns.  The weight is constant: its scales take no gradient.  It
     stays on its device (a module's ``to`` does not move it) and is in no ``state_dict``; it can be
     copied and pickled."""
 
@@ -235,6 +235,14 @@ def _once(backward):
     return lambda ctx_, dy: guarded(ctx_, dy) if torch.is_grad_enabled() else backward(ctx_, dy)
 
 
+def _linear_in(f, dy):
+    """f(dy) of a linear f, with its tangent where dy has one (forward mode over a backward pass)."""
+    if forward_ad._current_level < 0:
+        return f(dy)
+    dy, tangent = forward_ad.unpack_dual(dy)
+    return f(dy) if tangent is None else forward_ad.make_dual(f(dy), f(tangent))
+
+
 class _Int4LinearFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx_, x, weight, bias):
@@ -245,8 +253,8 @@ class _Int4LinearFn(torch.autograd.Function):
     @_once
     def backward(ctx_, dy):
         w = ctx_.weight
-        dx = w._product(dy, None, True) if ctx_.needs_input_grad[0] else None
-        db = _col_sum(_rows(dy, w.shape[0])) if ctx_.needs_input_grad[2] else None
+        dx = _linear_in(lambda d: w._product(d, None, True), dy) if ctx_.needs_input_grad[0] else None
+        db = _linear_in(lambda d: _col_sum(_rows(d, w.shape[0])), dy) if ctx_.needs_input_grad[2] else None
         return dx, None, db
 
 
@@ -301,6 +309,18 @@ def _lookup(ids, table, scale):
     return out
 
 
+def _table_grad(ids, dy, shape, scale, padding):
+    vocab, hidden = shape
+    d2 = _rows(dy, hidden)
+    index = dy.device.index
+    ctx = _lib.ctx_handle(index)
+    ws = _scratch("llmc_embedding_grad_workspace", index, dy.device, ids.numel(), vocab, hidden)
+    out = torch.empty(vocab, hidden, dtype=dy.dtype, device=dy.device)
+    _lib.call("llmc_embedding_grad", ctx, _lib.stream(index), ids.data_ptr(), int(ids.dtype == torch.int64), ids.numel(),
+              d2.data_ptr(), _DTYPES[dy.dtype], _pitch(d2), vocab, hidden, scale, padding, out.data_ptr(), ws.data_ptr(), ws.numel())
+    return out
+
+
 class _EmbeddingFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx_, table, ids, scale, padding):
@@ -312,16 +332,7 @@ class _EmbeddingFn(torch.autograd.Function):
     @_once
     def backward(ctx_, dy):
         (ids,) = ctx_.saved_tensors
-        vocab, hidden = ctx_.shape
-        d2 = _rows(dy, hidden)
-        index = dy.device.index
-        ctx = _lib.ctx_handle(index)
-        ws = _scratch("llmc_embedding_grad_workspace", index, dy.device, ids.numel(), vocab, hidden)
-        out = torch.empty(vocab, hidden, dtype=dy.dtype, device=dy.device)
-        _lib.call("llmc_embedding_grad", ctx, _lib.stream(index), ids.data_ptr(), int(ids.dtype == torch.int64), ids.numel(),
-                  d2.data_ptr(), _DTYPES[dy.dtype], _pitch(d2), vocab, hidden, ctx_.scale, ctx_.padding, out.data_ptr(),
-                  ws.data_ptr(), ws.numel())
-        return out, None, None, None
+        return _linear_in(lambda d: _table_grad(ids, d, ctx_.shape, ctx_.scale, ctx_.padding), dy), None, None, None
 
 
 def embedding(ids: torch.Tensor, table, scale: float = 1.0, padding_idx: int | None = None,

@@ -160,3 +160,45 @@ def test_compiled_callers_run_the_kernels():
     xs = x.clone().requires_grad_(True)
     (dx,) = torch.autograd.grad(torch.compile(lambda x: int4_linear(x * 2, p).sum(), backend="eager")(xs), xs)
     assert torch.equal(dx, torch.autograd.grad(int4_linear(xs * 2, p).sum(), xs)[0])
+
+
+def test_forward_mode_over_a_backward_pass(case, monkeypatch):
+    """The product of a second derivative with a vector: of sum (x W^T + b)^2 it is 2 (v W^T) W, and for b 2 sum v W^T."""
+    from llmcompressorsharp_b200 import int4_linear, packed
+
+    monkeypatch.setattr(packed, "_col_sum", lambda d: torch.tensor(d.tolist()).sum(0))
+    p, w, x, b, g = case
+    v = torch.randn(3, 7, generator=g)
+    x, b = x.requires_grad_(True), b.requires_grad_(True)
+    with forward_ad.dual_level():
+        xs = forward_ad.make_dual(x, v)
+        dx, db = torch.autograd.grad(int4_linear(xs, p, b).pow(2).sum(), [xs, b])
+        dx, hx = forward_ad.unpack_dual(dx)
+        db, hb = forward_ad.unpack_dual(db)
+    y = x @ w.t() + b
+    assert torch.allclose(dx, 2 * y @ w, atol=1e-4) and torch.allclose(db, 2 * y.sum(0), atol=1e-4)
+    assert torch.allclose(hx, 2 * (v @ w.t()) @ w, atol=1e-4) and torch.allclose(hb, 2 * (v @ w.t()).sum(0), atol=1e-4)
+
+
+@pytest.mark.gpu
+def test_forward_mode_over_a_backward_pass_on_the_device():
+    from llmcompressorsharp_b200 import embedding, int4_linear
+
+    e, w = entry(70, 130, group=64, pow2=True, device=ROOT_DEV)
+    p, w = weight(e, 130), w.float().to(ROOT_DEV)
+    g = torch.Generator().manual_seed(1)
+    x, v = (torch.randint(-3, 4, (9, 130), generator=g).float().to(ROOT_DEV) for _ in range(2))
+    table, u = (torch.randint(-3, 4, (11, 16), generator=g).float().to(ROOT_DEV) for _ in range(2))
+    b = torch.zeros(70, device=ROOT_DEV, requires_grad=True)
+    ids = torch.randint(0, 11, (40,), generator=g).to(ROOT_DEV)
+    x.requires_grad_(True), table.requires_grad_(True)
+    with forward_ad.dual_level():
+        xs, ts = forward_ad.make_dual(x, v), forward_ad.make_dual(table, u)
+        got = [forward_ad.unpack_dual(d).tangent for d in torch.autograd.grad((int4_linear(xs, p, b).pow(2)).sum(), [xs, b])]
+        got.append(forward_ad.unpack_dual(torch.autograd.grad(embedding(ids, ts, 2.0).pow(2).sum(), ts)[0]).tangent)
+    s = (v.double() @ w.double().t())
+    want = [2 * s @ w.double(), 2 * s.sum(0), 8 * u.double() * torch.bincount(ids, minlength=11)[:, None]]
+    # s is exact (integers times powers of two); a sum of n terms is off by 2^-23 of its absolute terms for each and 8 more
+    bounds = [78 * 2.0 ** -23 * (2 * s.abs() @ w.double().abs()), 17 * 2.0 ** -23 * 2 * s.abs().sum(0), torch.zeros(())]
+    for a, c, bound in zip(got, want, bounds):
+        assert bool(((a.double() - c).abs() <= bound.to(a.device)).all())
