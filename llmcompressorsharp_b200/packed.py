@@ -50,27 +50,27 @@ def _pitch(t: torch.Tensor) -> int:
     return t.stride(0) if t.shape[0] > 1 else max(1, t.shape[1])
 
 
-def _seen_by_torch(*tensors) -> str | None:
-    """What of torch's watches the operators that are run on these tensors, if anything does: a trace of the library's
-    calls would hold empty tensors in place of their results, a transform would lose its part of them."""
-    if torch._C._is_tracing():
-        return "torch.jit's tracing"
-    if torch._C._functorch.peek_interpreter_stack() is not None:
-        if any(isinstance(t, torch.Tensor) and torch._C._functorch.is_functorch_wrapped_tensor(t) for t in tensors):
-            return "a torch.func transform"
-    if torch._C._len_torch_dispatch_stack() and torch._C._get_dispatch_mode(torch._C._TorchDispatchModeKey.PROXY) is not None:
-        return "torch.fx's tracing"
-    for t in tensors:
-        if isinstance(t, torch.Tensor) and type(t) is not torch.Tensor and type(t) is not torch.nn.Parameter:
-            from torch._subclasses import FakeTensor
-
-            if isinstance(t, FakeTensor):
-                return "a FakeTensor"
-    return None
+_is_tracing, _transform, _modes = torch._C._is_tracing, torch._C._functorch.peek_interpreter_stack, torch._C._len_torch_dispatch_stack
 
 
-def _refuse_unseen(name: str, *tensors):
-    what = _seen_by_torch(*tensors)
+def _refuse_unseen(name: str, a, b):
+    """Refuses a call whose operators torch watches: a trace of the library's calls would hold empty tensors in place of
+    their results, a transform would lose its part of them.  (0.3 us where nothing does.)"""
+    if not (_is_tracing() or _modes()) and _transform() is None and type(a) in _PLAIN and type(b) in _PLAIN:
+        return
+    tensors = [t for t in (a, b) if isinstance(t, torch.Tensor)]
+    what = None
+    if _is_tracing():
+        what = "torch.jit's tracing"
+    elif any(torch._C._functorch.is_functorch_wrapped_tensor(t) for t in tensors):
+        what = "a torch.func transform"
+    elif _modes() and torch._C._get_dispatch_mode(torch._C._TorchDispatchModeKey.PROXY) is not None:
+        what = "torch.fx's tracing"
+    else:
+        from torch._subclasses import FakeTensor
+
+        if any(isinstance(t, FakeTensor) for t in tensors):
+            what = "a FakeTensor"
     if what is not None:
         raise NotSupportedError(f"{name} cannot run under {what}: its kernels are not torch operators")
 
@@ -202,6 +202,8 @@ class Int4Weight:
         return out
 
 
+# What the calls get outside torch's transforms and traces; they look closer at anything else.
+_PLAIN = frozenset((torch.Tensor, torch.nn.Parameter, Int4Weight, type(None)))
 _needs: dict = {}  # (call, device, sizes) -> bytes of scratch
 
 
@@ -442,8 +444,8 @@ class TokenEmbedding(torch.nn.Embedding):
         if (w.is_cuda and w.dtype in _DTYPES and ids.dtype in (torch.int64, torch.int32) and type(ids) is torch.Tensor
                 and type(w) in (torch.Tensor, torch.nn.Parameter)
                 and self.max_norm is None and not self.scale_grad_by_freq and not self.sparse
-                and forward_ad._current_level < 0 and not torch.compiler.is_compiling() and not torch._C._is_tracing()
-                and torch._C._functorch.peek_interpreter_stack() is None and not torch._C._len_torch_dispatch_stack()):
+                and forward_ad._current_level < 0 and not torch.compiler.is_compiling() and not _is_tracing()
+                and _transform() is None and not _modes()):
             return embedding(ids, w, padding_idx=self.padding_idx)
         return super().forward(ids)
 
