@@ -132,6 +132,8 @@ class Context {
     int device() const { return device_; }
     // Waits for the context's stream and raises its first deferred device error.
     void Synchronize() const { Check(llmc_sync(ctx_)); }
+    // The same, but an embedding id outside its table stays pending (llmc_wait).
+    void Wait() const { Check(llmc_wait(ctx_)); }
     // Extensions (no reference counterpart): the stream the context's work is ordered on, an SM
     // cap for its persistent grids (0: the whole GPU), the tries of a bounded device wait
     // (negative: the default), device-side "not positive definite" decisions reported by

@@ -25,7 +25,8 @@ constexpr int64_t MAX_DIM = (int64_t)1 << 30;     // rows, columns, tokens
 // tensor-core kernel, which takes as long for 17 tokens as for 128, does not pass it.  us here and there, 16-bit: 4096 -> 14336,
 // 32 tokens 33 and 33, 48: 47 and 33; 4096 -> 4096, 32: 12.5 and 16.5, 64: 18.1 and 17.1; 576 -> 1536, 256: 11.5 and 14.
 // fp32 costs six products there and three here: 4096 -> 14336, 256: 373 and 489; 4096 -> 4096, 256: 114 and 127; with
-// few columns (not eight tiles) there is less to overlap: 576 -> 49152, 64: 117 and 118, 96: 172 and 122.
+// few columns (not eight tiles) there is less to overlap: 576 -> 49152, 64: 117 and 118, 96: 172 and 122.  The borders lie
+// between these shapes; others near them may be up to a third slower on the side that they are given.
 bool few_rows(bool f32, int64_t tokens, int64_t rows, int64_t cols) {
     if (tokens <= (f32 ? 64 : 32)) return true;
     if (tokens > 256) return false;

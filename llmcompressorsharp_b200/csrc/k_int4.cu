@@ -251,10 +251,12 @@ __device__ __forceinline__ void copy16(void* dst, const void* src, int bytes) { 
 // add their sums in shared memory, in warp order.  Each warp keeps a ring of STAGES steps, the records and the 256 bytes
 // a tile of each token's x (XS), by 16-byte asynchronous copies that it waits for by itself.  The three pieces of fp32
 // x would take most of the ring and are read through L1, which row blocks of few columns share.
-// What bounds it is the instructions: at the HBM's rate an SM has 43 clocks for a record, 172 issue slots, of which
-// turning its codes into numbers takes 88 and the rest of its arithmetic 26; loops, copies and waits take about 70 more.
-// One token, bf16: 14336 -> 4096 11.5 us (2.8 TB/s; two instructions a clock of four, 256 CTAs on 148 SMs), 576 -> 576 2.3,
-// 4096 -> 14336 12.4.  16 tokens 18.
+// What bounds it is latency and balance.  A record's instructions (88 to turn its codes into numbers, 26 of other
+// arithmetic, about 70 of loops, copies and waits) are 1.06 times the issue slots that an SM has for it at the HBM's rate,
+// and one token of 14336 -> 4096 takes 2.4 times that: a scheduler's three or four warps, each one chain of load, mask,
+// subtract, multiply, scale, leave 48 % of its slots empty, and an SM is active 0.66 of the time (256 CTAs on 148 SMs, start
+// and end).  One token, bf16: 14336 -> 4096 11.5 us (2.8 TB/s), 576 -> 576 2.3, 4096 -> 14336 12.4.  16 tokens 18 (2.3 warps
+// to a scheduler, 64 % of the slots empty).
 template <typename T, typename O, int NT, int PIECES, int NG, int RB>
 __global__ void __launch_bounds__(32 * FEW_WARPS) few_kernel(const FewArgs a) {
     constexpr int REC = 1024 + 80 * NG, FL = 4 / NG, SUMS = 8 * NT * ROWS * RB, STAGES = few_stages(NT, RB), FEW_TILES = few_tiles(NT, RB);

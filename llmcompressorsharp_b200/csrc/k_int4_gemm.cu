@@ -32,11 +32,12 @@
 // A stage is a whole tile, 128 of the contraction: the MMA warp's two waits and its commit take some hundreds of
 // clocks, which the MMAs of 64 (512 clocks) did not cover.
 //
-// 4096 -> 14336, 8,192 tokens, bf16: 735 to 760 us in short runs (1.3 PFLOP/s; the library's product of a 16-bit weight 648),
+// 4096 -> 14336, 8,192 tokens, bf16: 735 to 775 us in short runs (1.25 to 1.3 PFLOP/s; the library's product of a 16-bit weight 648),
 // 860 back to back at the power limit (731); 813 in short runs with one thread issuing the MMAs inside a branch and
 // building its descriptors each time.  2,048 tokens of 4096 -> 4096: 68 us back to back (53), its gradient 66.  At 33 to 128
 // tokens the eight warps that dequantise bound it: 29 us for 4096 -> 14336, where the codes alone are read in 5.  Numbers
-// made before the wait for a free stage instead of behind it: no faster.
+// made before the wait for a free stage instead of behind it: no faster.  fp32, 2,048 tokens of 4096 -> 4096: 937 us, its
+// gradient 905 (0.31 of the rate of six bf16 products).
 // Every wait is bounded.
 //
 // What orders the rings, each turn of a slot by one phase of its barriers:
@@ -659,7 +660,8 @@ llmc_status launch(llmc_ctx* ctx, cudaStream_t st, const CUtensorMap& map, GemmI
 // CTAs per tile: pairs (256 x 256) share what they dequantise and load, single CTAs (128 x 128) fill more SMs, so they are
 // taken while one round of them holds the product and the contraction is not so long that sharing counts for more.  us, fp16,
 // single and pairs: 4096 -> 4096, 512 tokens (128 tiles) 33 and 38, 768 (192) 54 and 41; 2048 -> 2048, 1,024 (128) 21 and 32,
-// 2,048 (256) 34 and 29; 576 -> 1536, 1,024 (96) 12 and 25; 14336 -> 4096, 160 tokens 52 and 42, 512 86 and 76.
+// 2,048 (256) 34 and 29; 576 -> 1536, 1,024 (96) 12 and 25; 14336 -> 4096, 160 tokens 52 and 42, 512 86 and 76.  Contractions
+// between 4,096 and 14,336 were not measured: the border is their geometric middle, rounded.
 int int4_gemm_cg(const llmc_ctx* ctx, int dtype, int64_t tokens, int64_t cols, int64_t contraction) {
     if (dtype == LLMC_DTYPE_F32 || tokens <= 128 || cols <= 128) return 1;
     const bool round = (tokens + 127) / 128 * ((cols + 127) / 128) <= ctx->sm_count;
